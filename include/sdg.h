@@ -292,6 +292,56 @@ SDG_API int sdg_upsample_conv3x3(const uint16_t* x, int B, int H, int W, int Ci,
                                  const float* bias4, int Co, uint16_t* y, void* workspace, size_t workspace_bytes,
                                  int* err_word, void* stream);
 
+/* --- 4-bit microscaled operands (MXFP4) ---------------------------------------------
+ * No reference counterpart: the reference quantises weights only, to int8 (tools/quantize_wo8.py).
+ * A matrix [R, K] in MXFP4 (OCP Microscaling Formats 1.0: E2M1 values, one E8M0 exponent per 32
+ * consecutive columns of a row) is two device arrays, both 16-byte aligned:
+ *   codes  [R][Kp/2], Kp = K rounded up to 32: two values a byte, the even column in the low nibble,
+ *          zero codes behind column K;
+ *   scales [ceil(R/128)][ceil(Kp/128)][512]: the biased exponent of row r, block b (columns 32b..) is byte
+ *          (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of tile (r / 128, b / 4); bytes of no block are zero.
+ * Quantisation of a block: exponent e = max(floor(log2(max|x|)) - 2, -127), codes = x / 2^e rounded to
+ * nearest even and saturated at +-6; a block holding an infinity or a NaN gets the exponent NaN (255) and
+ * reads back as 32 NaNs. An operand serves as activations (x) or as weights (w, one row per output). */
+enum { SDG_F16 = 0, SDG_BF16 = 1, SDG_F32 = 2 }; /* element types of the functions below */
+
+/* Bytes of the two arrays of an [R, K] operand (0 on bad input). */
+SDG_API size_t sdg_mx4_code_bytes(int R, int K);
+SDG_API size_t sdg_mx4_scale_bytes(int R, int K);
+
+/* x [R, K] (dtype any of the three, row stride ldx elements, any K >= 1) -> codes, scales. Writes every
+ * byte of both arrays. */
+SDG_API int sdg_quantize_mx4(const void* x, int dtype, int R, int K, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                             void* stream);
+
+/* The values an operand stands for: y [R, K] contiguous, rounded once to dtype. */
+SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int R, int K, int dtype, void* y,
+                               void* stream);
+
+/* y[M,N] = act(x w^T + bias + residual) for MXFP4 x [M, K] and w [N, K], fp32 accumulation. bias [N] fp32
+ * (may be NULL); residual [M, N] and y of type dtype (SDG_F16 or SDG_BF16), 16-byte aligned; y may be the
+ * residual itself. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of 16 as for sdg_linear,
+ * y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above. */
+SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
+                           const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,
+                           void* y, int* err_word, void* stream);
+
+/* The same with x [M, K] of type dtype (row stride ldx elements), quantised on the way into scratch
+ * (sdg_linear_mx4_scratch_bytes(M, K) bytes, 16-byte aligned; its contents on entry do not matter). */
+SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales,
+                             const float* bias, int N, const void* residual, int act, int dtype, void* y, void* scratch,
+                             size_t scratch_bytes, int* err_word, void* stream);
+SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K);
+
+/* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
+ * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to
+ * 16 bits in between. C a multiple of 8 and of groups. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
+ * of device memory, any contents. Deterministic; an image's result does not depend on the batch. */
+SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, int groups, const float* gamma,
+                              const float* beta, float eps, int silu, uint8_t* codes, uint8_t* scales,
+                              float* stats_scratch, void* stream);
+SDG_API size_t sdg_groupnorm_mx4_scratch_bytes(int B, int HW, int C, int groups);
+
 #ifdef __cplusplus
 }
 #endif

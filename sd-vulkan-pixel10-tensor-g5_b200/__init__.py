@@ -97,6 +97,15 @@ _SIGS = {
     "sdg_concat": (_I, [_P, _I, _P, _I, _I, _P, _P]),
     "sdg_upsample2x": (_I, [_P, _I, _I, _I, _I, _P, _P]),
     "sdg_pack_upsample_conv_weights": (_I, [_P, _I, _I, _P]),
+    "sdg_mx4_code_bytes": (ctypes.c_size_t, [_I, _I]),
+    "sdg_mx4_scale_bytes": (ctypes.c_size_t, [_I, _I]),
+    "sdg_quantize_mx4": (_I, [_P, _I, _I, _I, ctypes.c_int64, _P, _P, _P]),
+    "sdg_dequantize_mx4": (_I, [_P, _P, _I, _I, _I, _P, _P]),
+    "sdg_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P]),
+    "sdg_linear_mx4_x": (_I, [_P, _I, _I, ctypes.c_int64, _P, _P, _P, _I, _P, _I, _I, _P, _P, ctypes.c_size_t, _P, _P]),
+    "sdg_linear_mx4_scratch_bytes": (ctypes.c_size_t, [_I, _I]),
+    "sdg_groupnorm_mx4": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
+    "sdg_groupnorm_mx4_scratch_bytes": (ctypes.c_size_t, [_I, _I, _I, _I]),
     "sdg_upsample_conv3x3": (_I, [_P, _I, _I, _I, _I, _P, _P, _I, _P, _P, ctypes.c_size_t, _P, _P]),
 }
 
@@ -446,6 +455,198 @@ def upsample_conv3x3(x, wp, bias4, out=None, workspace=None, err_word=None, stre
     check(lib().sdg_upsample_conv3x3(_ptr(x), B, H, W, Ci, _ptr(wp), _ptr(bias4), Co, _ptr(out), _ptr(workspace), wsb,
                                      _ptr(err_word), _stream(stream)))
     return out
+
+
+# ------------------------------------------------------------------ 4-bit microscaled operands (MXFP4)
+# A matrix [rows, K] is (codes, scales): codes uint8 [rows, Kp/2] (Kp = K rounded up to 32), scales uint8
+# [ceil(rows/128), ceil(Kp/128), 512]; the layout is described in include/sdg.h. Every tensor of a call lives on
+# one CUDA device, which need not be the current one; the call runs on that device's current stream, or on
+# ``stream`` (a raw handle of a stream of that device).
+_mx4_types: Dict[object, int] = {}
+
+
+def _mx4_dtype(dt, wide: bool = True) -> int:
+    if not _mx4_types:
+        import torch
+        _mx4_types.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    code = _mx4_types.get(dt, 3)
+    if code > (2 if wide else 1):
+        raise SdgError(2, f"MXFP4 operators take fp16, bf16{' or fp32' if wide else ''} tensors, not {dt}")
+    return code
+
+
+def _mx4_arg(t, name: str, dev, dtype=None, shape=None):
+    """Checks one tensor argument; returns its device pointer (None for a missing one)."""
+    if t is None:
+        return None
+    if t.device != dev or (dtype is not None and t.dtype != dtype):
+        raise SdgError(2, f"{name}: expected {dtype or t.dtype} on {dev}, got {t.dtype} on {t.device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise SdgError(3, f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
+    if not t.is_contiguous():
+        raise SdgError(2, f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _mx4_device(t):
+    if not t.is_cuda:
+        raise SdgError(2, "MXFP4 operators take CUDA tensors")
+    return t.device
+
+
+def _mx4_scale_shape(rows: int, half: int):
+    return ((rows + 127) // 128, (half + 63) // 64, 512)
+
+
+def _mx4_call(fn, dev, stream, fresh, *args) -> None:
+    """Runs one C entry on ``dev``; ``fresh``: tensors allocated by this call (from the current stream's pool),
+    which must not be reused before the work on another ``stream`` is done."""
+    import torch
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _mx4_call(fn, dev, stream, fresh, *args)
+    if stream is None:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index) or None))
+        return
+    try:
+        check(fn(*args, stream or None))
+    finally:
+        side = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+        for t in fresh:
+            t.record_stream(side)
+
+
+def _mx4_empty(rows: int, half: int, dev):
+    import torch
+    return (torch.empty((rows, half), dtype=torch.uint8, device=dev),
+            torch.empty(_mx4_scale_shape(rows, half), dtype=torch.uint8, device=dev))
+
+
+def _mx4_rows(x):
+    """(rows, K, row stride) of a 2-D tensor whose rows are contiguous."""
+    if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 1:
+        raise SdgError(3, f"expected a matrix with at least one row and column, got {list(x.shape)}")
+    R, K = x.shape
+    if K > 1 and x.stride(1) != 1:
+        raise SdgError(2, "the columns of a row must be contiguous")
+    return R, K, x.stride(0) if R > 1 else K
+
+
+def quantize_mx4(x, out=None, stream=None):
+    """x [rows, K] fp16 / bf16 / fp32 (rows may be strided) -> (codes, scales) in MXFP4. ``out``: the pair to
+    write into. Weights [N, K] and activations [M, K] are quantised alike."""
+    import torch
+    dev = _mx4_device(x)
+    dt = _mx4_dtype(x.dtype)
+    R, K, ldx = _mx4_rows(x)
+    half = (K + 31) // 32 * 16
+    codes, scales = out if out is not None else _mx4_empty(R, half, dev)
+    pc = _mx4_arg(codes, "codes", dev, torch.uint8, (R, half))
+    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(R, half))
+    _mx4_call(lib().sdg_quantize_mx4, dev, stream, () if out is not None else (codes, scales), x.data_ptr(), dt, R, K,
+              ldx, pc, ps)
+    return codes, scales
+
+
+def dequantize_mx4(codes, scales, K: Optional[int] = None, dtype=None, out=None, stream=None):
+    """The values an MXFP4 operand stands for, [rows, K] (all Kp columns when K is None), as ``dtype`` (fp16)."""
+    import torch
+    dev = _mx4_device(codes)
+    if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] < 16 or codes.shape[1] % 16:
+        raise SdgError(3, f"codes: expected [rows, Kp/2], got {list(codes.shape)}")
+    R, half = codes.shape
+    K = 2 * half if K is None else K
+    if not 2 * half - 32 < K <= 2 * half:
+        raise SdgError(3, f"K = {K} does not fit codes of {2 * half} columns")
+    pc = _mx4_arg(codes, "codes", dev, torch.uint8)
+    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(R, half))
+    fresh = ()
+    if out is None:
+        out = torch.empty((R, K), dtype=dtype or torch.float16, device=dev)
+        fresh = (out,)
+    py = _mx4_arg(out, "out", dev, dtype, (R, K))
+    _mx4_call(lib().sdg_dequantize_mx4, dev, stream, fresh, pc, ps, R, K, _mx4_dtype(out.dtype), py)
+    return out
+
+
+def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscale=None, dtype=None, out=None,
+               err_word=None, stream=None):
+    """y [M, N] = act(x w^T + bias + residual) with both operands in MXFP4 and fp32 accumulation. x is [M, K]
+    fp16 / bf16 (quantised on the way; y has its type), or the codes [M, Kp/2] of an operand whose scales are
+    ``xscale`` (y has ``dtype``, fp16 by default). w: ``quantize_mx4`` of the [N, K] weight; act 2 = GEGLU on rows
+    packed by ``pack_geglu_weight`` before quantising, y [M, N/2]. ``out`` may be the residual."""
+    import torch
+    dev = _mx4_device(x)
+    if wcodes.dim() != 2:
+        raise SdgError(3, f"wcodes: expected [N, Kp/2], got {list(wcodes.shape)}")
+    N, half = wcodes.shape
+    if xscale is None:
+        M, K, ldx = _mx4_rows(x)
+        dt = x.dtype
+        if dtype is not None and dtype != dt:
+            raise SdgError(2, f"y has the type of x, {dt}")
+        if half != (K + 31) // 32 * 16:
+            raise SdgError(3, f"x has {K} columns, the weight {2 * half}")
+    else:
+        if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] != half or half % 16:
+            raise SdgError(3, f"x codes: expected [M, {half}], got {list(x.shape)}")
+        M, K = x.shape[0], 2 * half
+        dt = dtype or torch.float16
+    code = _mx4_dtype(dt, wide=False)
+    pw = _mx4_arg(wcodes, "wcodes", dev, torch.uint8)
+    pws = _mx4_arg(wscales, "wscales", dev, torch.uint8, _mx4_scale_shape(N, half))
+    pb = _mx4_arg(bias, "bias", dev, torch.float32, (N,))
+    pr = _mx4_arg(residual, "residual", dev, dt, (M, N))
+    pe = _mx4_arg(err_word, "err_word", dev, torch.int32)
+    fresh = []
+    if out is None:
+        out = torch.empty((M, N // 2 if act == 2 else N), dtype=dt, device=dev)
+        fresh.append(out)
+        py = out.data_ptr()
+    else:
+        py = _mx4_arg(out, "out", dev, dt, (M, N // 2 if act == 2 else N))
+    if xscale is None:
+        nb = (M * half + 511) // 512 * 512 + ((M + 127) // 128) * ((half + 63) // 64) * 512
+        scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
+        fresh.append(scratch)
+        _mx4_call(lib().sdg_linear_mx4_x, dev, stream, fresh, x.data_ptr(), M, K, ldx, pw, pws, pb, N, pr, act, code, py,
+                  scratch.data_ptr(), nb, pe)
+    else:
+        px = _mx4_arg(x, "x codes", dev, torch.uint8)
+        pxs = _mx4_arg(xscale, "xscale", dev, torch.uint8, _mx4_scale_shape(M, half))
+        _mx4_call(lib().sdg_linear_mx4, dev, stream, fresh, px, pxs, M, K, pw, pws, pb, N, pr, act, code, py, pe)
+    return out
+
+
+def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=None, stats=None, stream=None):
+    """GroupNorm (+ SiLU) of channels-last x [B, HW, C] fp16 / bf16, quantised as it is written: the MXFP4 operand
+    (codes, scales) of the matrix [B * HW, C]. ``out``: the pair to write into."""
+    import torch
+    dev = _mx4_device(x)
+    if x.dim() != 3 or 0 in x.shape:
+        raise SdgError(3, f"x: expected [B, HW, C], got {list(x.shape)}")
+    B, HW, C = x.shape
+    dt = _mx4_dtype(x.dtype, wide=False)
+    px = _mx4_arg(x, "x", dev)
+    pg = _mx4_arg(gamma, "gamma", dev, torch.float32, (C,))
+    pb = _mx4_arg(beta, "beta", dev, torch.float32, (C,))
+    half = (C + 31) // 32 * 16
+    fresh = []
+    if out is None:
+        out = _mx4_empty(B * HW, half, dev)
+        fresh += out
+    codes, scales = out
+    pc = _mx4_arg(codes, "codes", dev, torch.uint8, (B * HW, half))
+    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(B * HW, half))
+    need = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups)
+    if stats is None:
+        stats = torch.empty((need // 4 + 1,), dtype=torch.float32, device=dev)
+        fresh.append(stats)
+    pt = _mx4_arg(stats, "stats", dev, torch.float32)
+    if stats.numel() * 4 < need:
+        raise SdgError(2, f"stats: {need} bytes are needed")
+    _mx4_call(lib().sdg_groupnorm_mx4, dev, stream, fresh, px, dt, B, HW, C, groups, pg, pb, eps, int(silu), pc, ps, pt)
+    return codes, scales
 
 
 # ------------------------------------------------------------------ engine weight layouts (for the op surface)

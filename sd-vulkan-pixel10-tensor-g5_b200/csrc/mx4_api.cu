@@ -1,0 +1,162 @@
+// mx4_api.cu — C entry points of the MXFP4 operators (include/sdg.h): quantise, read back, linear, GroupNorm
+// into an MXFP4 operand.
+#include <mutex>
+#include <string>
+
+#include "../../include/sdg.h"
+#include "mx4.cuh"
+#include "sdg_kernels.h"
+
+namespace sdg {
+int op_fail(int code, const std::string& msg);
+}
+
+namespace {
+
+using sdg::op_fail;
+
+// The word the kernels' bounded waits report to when the caller passes none: zero-initialised device memory of the
+// library, looked up once per device. The look-up may load the module, so it runs with this thread's
+// stream-capture mode relaxed: a first call inside a capture is fine.
+static __device__ int g_mx4_err[64];
+std::mutex g_mu;
+int* g_err_dev[64] = {nullptr};
+
+int* default_err_word() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_err_dev[dev]) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool swapped = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_mx4_err) == cudaSuccess) g_err_dev[dev] = static_cast<int*>(p);
+    if (swapped) cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+  return g_err_dev[dev];
+}
+
+int status(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return SDG_OK;
+  if (e == cudaErrorInvalidValue) return op_fail(SDG_ERR_SHAPE, std::string(what) + ": unsupported shape or arguments");
+  return op_fail(SDG_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+size_t elem_bytes(int dtype) { return dtype == sdg::kF32 ? 4 : 2; }
+// grid.y walks the 128-column scale tiles
+constexpr int kMaxK = 65535 * sdg::kMxTileCols;
+
+int linear_check(const char* what, int M, int K, const uint8_t* wcodes, const uint8_t* wscales, const float* bias, int N,
+                 const void* residual, int act, int dtype, const void* y) {
+  const std::string w(what);
+  if (!wcodes || !wscales || !y || M <= 0 || K <= 0 || N <= 0 || K > kMaxK || act < 0 || act > 2)
+    return op_fail(SDG_ERR_ARG, w + ": bad arguments");
+  if (dtype != sdg::kF16 && dtype != sdg::kBF16) return op_fail(SDG_ERR_ARG, w + ": dtype must be fp16 or bf16");
+  if (act == 2 && residual) return op_fail(SDG_ERR_ARG, w + ": GEGLU takes no residual");
+  if (act == 2 ? N % 32 : N % 8)
+    return op_fail(SDG_ERR_SHAPE, w + (act == 2 ? ": GEGLU needs N a multiple of 32" : ": N must be a multiple of 8"));
+  if (!aligned(wcodes, 16) || !aligned(wscales, 16) || !aligned(y, 16) || !aligned(residual, 16) || !aligned(bias, 4))
+    return op_fail(SDG_ERR_ARG, w + ": weight, scale, residual and output pointers must be 16-byte aligned");
+  return SDG_OK;
+}
+
+int linear_run(const char* what, const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
+               const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype, void* y,
+               int* err_word, cudaStream_t s) {
+  sdg::Mx4LinearArgs a;
+  a.xcodes = xcodes; a.xscales = xscales; a.wcodes = wcodes; a.wscales = wscales;
+  a.M = M; a.N = N; a.K = K; a.bias = bias; a.residual = residual; a.act = act; a.dtype = dtype; a.y = y;
+  int* err = err_word ? err_word : default_err_word();
+  if (!err) return op_fail(SDG_ERR_CUDA, std::string(what) + ": no device error word");
+  return status(sdg::launch_mx4_linear(a, err, s), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+SDG_API size_t sdg_mx4_code_bytes(int M, int K) {
+  return M <= 0 || K <= 0 || K > kMaxK ? 0 : (size_t)M * (sdg::mx_kp(K) / 2);
+}
+SDG_API size_t sdg_mx4_scale_bytes(int M, int K) {
+  return M <= 0 || K <= 0 || K > kMaxK ? 0 : (size_t)sdg::mx_rtiles(M) * sdg::mx_ktiles(K) * sdg::kMxTileBytes;
+}
+
+SDG_API int sdg_quantize_mx4(const void* x, int dtype, int M, int K, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                             void* stream) {
+  if (!x || !codes || !scales || M <= 0 || K <= 0 || K > kMaxK || ldx < 0)
+    return op_fail(SDG_ERR_ARG, "quantize_mx4: bad arguments");
+  if (dtype < sdg::kF16 || dtype > sdg::kF32) return op_fail(SDG_ERR_ARG, "quantize_mx4: dtype must be fp16, bf16 or fp32");
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(x, elem_bytes(dtype)))
+    return op_fail(SDG_ERR_ARG, "quantize_mx4: codes and scales must be 16-byte aligned, x aligned to its type");
+  return status(sdg::launch_mx4_quantize(x, dtype, M, K, ldx, codes, scales, static_cast<cudaStream_t>(stream)),
+                "quantize_mx4");
+}
+
+SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int M, int K, int dtype, void* y,
+                               void* stream) {
+  if (!y || !codes || !scales || M <= 0 || K <= 0 || K > kMaxK)
+    return op_fail(SDG_ERR_ARG, "dequantize_mx4: bad arguments");
+  if (dtype < sdg::kF16 || dtype > sdg::kF32)
+    return op_fail(SDG_ERR_ARG, "dequantize_mx4: dtype must be fp16, bf16 or fp32");
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(y, elem_bytes(dtype)))
+    return op_fail(SDG_ERR_ARG, "dequantize_mx4: codes and scales must be 16-byte aligned, y aligned to its type");
+  return status(sdg::launch_mx4_dequantize(codes, scales, M, K, dtype, y, static_cast<cudaStream_t>(stream)),
+                "dequantize_mx4");
+}
+
+SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
+                           const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,
+                           void* y, int* err_word, void* stream) {
+  int st = linear_check("linear_mx4", M, K, wcodes, wscales, bias, N, residual, act, dtype, y);
+  if (st) return st;
+  if (!xcodes || !xscales || !aligned(xcodes, 16) || !aligned(xscales, 16))
+    return op_fail(SDG_ERR_ARG, "linear_mx4: x codes and scales must be 16-byte aligned device pointers");
+  return linear_run("linear_mx4", xcodes, xscales, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word,
+                    static_cast<cudaStream_t>(stream));
+}
+
+SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales,
+                             const float* bias, int N, const void* residual, int act, int dtype, void* y, void* scratch,
+                             size_t scratch_bytes, int* err_word, void* stream) {
+  int st = linear_check("linear_mx4", M, K, wcodes, wscales, bias, N, residual, act, dtype, y);
+  if (st) return st;
+  const size_t cb = (sdg_mx4_code_bytes(M, K) + 511) / 512 * 512;
+  if (!x || ldx < 0 || !scratch || !aligned(scratch, 16) || !aligned(x, 2) || scratch_bytes < cb + sdg_mx4_scale_bytes(M, K))
+    return op_fail(SDG_ERR_ARG, "linear_mx4: bad x, or scratch smaller than sdg_linear_mx4_scratch_bytes");
+  uint8_t* xc = static_cast<uint8_t*>(scratch);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  st = status(sdg::launch_mx4_quantize(x, dtype, M, K, ldx, xc, xc + cb, s), "linear_mx4");
+  if (st) return st;
+  return linear_run("linear_mx4", xc, xc + cb, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word, s);
+}
+
+SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K) {
+  return (sdg_mx4_code_bytes(M, K) + 511) / 512 * 512 + sdg_mx4_scale_bytes(M, K);
+}
+
+SDG_API size_t sdg_groupnorm_mx4_scratch_bytes(int B, int HW, int C, int groups) {
+  if (B <= 0 || HW <= 0 || C <= 0 || groups <= 0) return 0;
+  return sdg::mx4_groupnorm_scratch_bytes(B, HW, C, groups);
+}
+
+SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, int groups, const float* gamma,
+                              const float* beta, float eps, int silu, uint8_t* codes, uint8_t* scales,
+                              float* stats_scratch, void* stream) {
+  if (!x || !gamma || !beta || !codes || !scales || !stats_scratch || B <= 0 || HW <= 0 || C <= 0 || groups <= 0)
+    return op_fail(SDG_ERR_ARG, "groupnorm_mx4: bad arguments");
+  if (dtype != sdg::kF16 && dtype != sdg::kBF16) return op_fail(SDG_ERR_ARG, "groupnorm_mx4: dtype must be fp16 or bf16");
+  if (C % 8 || C % groups || C > kMaxK || B > 65535 || (int64_t)B * HW > INT32_MAX)
+    return op_fail(SDG_ERR_SHAPE, "groupnorm_mx4: C must be a multiple of 8 and of groups, B at most 65535, B * HW below 2^31");
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(stats_scratch, 8) || !aligned(gamma, 4) ||
+      !aligned(beta, 4))
+    return op_fail(SDG_ERR_ARG, "groupnorm_mx4: x, codes and scales must be 16-byte aligned");
+  sdg::Mx4GroupNormArgs a;
+  a.x = x; a.dtype = dtype; a.B = B; a.HW = HW; a.C = C; a.groups = groups;
+  a.gamma = gamma; a.beta = beta; a.eps = eps; a.silu = silu;
+  a.codes = codes; a.scales = scales; a.stats = stats_scratch;
+  return status(sdg::launch_mx4_groupnorm(a, static_cast<cudaStream_t>(stream)), "groupnorm_mx4");
+}
+
+}  // extern "C"

@@ -127,6 +127,38 @@ struct AttnArgs {
 };
 cudaError_t launch_attention(const AttnArgs& a, int* dev_err, cudaStream_t s);
 
+// MXFP4 operands (format: mx4.cuh): codes [rows][Kp/2], scales [ceil(rows/128)][ceil(Kp/128)][512].
+enum ElemType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
+// x [M, K] with row stride ldx (elements) -> operand. Writes every byte of both arrays.
+cudaError_t launch_mx4_quantize(const void* x, int dtype, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales,
+                                cudaStream_t s);
+// operand -> y [M, K], contiguous.
+cudaError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, int dtype, void* y,
+                                  cudaStream_t s);
+// y = act(x w^T + bias + residual): x [M, K], w [N, K] MXFP4, y [M, N] (act 2, GEGLU: [M, N/2], w rows and bias
+// interleaved 16 value / 16 gate as for kEpiGeglu); residual and y of type dtype (kF16 or kBF16).
+struct Mx4LinearArgs {
+  const uint8_t* xcodes = nullptr; const uint8_t* xscales = nullptr;
+  const uint8_t* wcodes = nullptr; const uint8_t* wscales = nullptr;
+  int M = 0, N = 0, K = 0;
+  const float* bias = nullptr; const void* residual = nullptr;
+  int act = 0, dtype = kF16;
+  void* y = nullptr;
+};
+cudaError_t launch_mx4_linear(const Mx4LinearArgs& a, int* dev_err, cudaStream_t s);
+// GroupNorm (+ SiLU) of channels-last x [B, HW, C] (kF16 or kBF16) -> operand [B * HW, C]. stats:
+// mx4_groupnorm_scratch_bytes() bytes.
+struct Mx4GroupNormArgs {
+  const void* x = nullptr;
+  int dtype = kF16, B = 1, HW = 1, C = 0, groups = 32;
+  const float* gamma = nullptr; const float* beta = nullptr;
+  float eps = 1e-5f; int silu = 0;
+  uint8_t* codes = nullptr; uint8_t* scales = nullptr;
+  float* stats = nullptr;
+};
+cudaError_t launch_mx4_groupnorm(const Mx4GroupNormArgs& a, cudaStream_t s);
+size_t mx4_groupnorm_scratch_bytes(int B, int HW, int C, int groups);
+
 // small kernels (sdg_misc.cu)
 cudaError_t launch_time_embedding(const float* timesteps, int n_t, int B, const float* temb_proj_in, float* out320,
                                   cudaStream_t s);
