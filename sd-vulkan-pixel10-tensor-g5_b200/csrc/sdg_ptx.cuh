@@ -329,6 +329,55 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) 
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// ------------------------------------------------------------------ bulk copies and TMA stores (no multicast)
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) counted on an mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const void* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's newest store groups may still be reading shared memory.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------ block-scaled 4-bit MMA
+// D[tmem] (+)= (A * scaleA) (B * scaleB)^T, kind::mxf4: E2M1 operands (K = 64 per instruction), one E8M0 scale
+// per 32 values of K, read from TMEM.
+__device__ __forceinline__ void mma_mxf4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+// 32 rows x 16 bytes of shared memory (512 contiguous bytes) -> 32 TMEM lanes x 4 columns, repeated in all four
+// lane quadrants: one tile of scales. Executes in order with the MMAs that the same thread issues.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Descriptor of such a tile: no swizzle, 8-row groups of 128 bytes.
+__device__ __forceinline__ uint64_t sdesc_scales(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+// Instruction descriptor, kind::mxf4: [4,6) scale id of B, [7,10) A format (1 = E2M1), [10,12) B format, [17,23) N>>3,
+// 23 scale format (1 = E8M0), [27,29) M>>7, [29,31) scale id of A. The scale id (0 or 2) is the first of the two bytes
+// that the instruction takes from each 4-byte scale column.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, uint32_t scale_id) {
+  return (scale_id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(M >> 7) << 27) | (scale_id << 29);
+}
+
 // ------------------------------------------------------------------ small math
 // SiLU(x) = x * sigmoid(x) = x * (1/2 + tanh(x/2)/2): one MUFU instruction (tanh.approx) per value
 __device__ __forceinline__ float tanh_approx(float x) {
