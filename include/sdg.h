@@ -335,7 +335,7 @@ SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K);
 
 /* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
  * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to
- * 16 bits in between. C a multiple of 8 and of groups. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
+ * 16 bits in between. C a multiple of 8 and of groups, at most 4096. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
  * of device memory, any contents. Deterministic; an image's result does not depend on the batch. */
 SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, int groups, const float* gamma,
                               const float* beta, float eps, int silu, uint8_t* codes, uint8_t* scales,

@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <cstdint>
 
+#include "sdg_ptx.cuh"
+
 namespace sdg {
 
 constexpr int kMxBlock = 32;        // columns per exponent
@@ -72,32 +74,33 @@ __device__ __forceinline__ void mx_decode8(uint32_t c, __half2 (&h)[4]) {
   for (int i = 0; i < 4; ++i) h[i] = reinterpret_cast<__half2&>(r[i]);
 }
 
-// max |v| of eight values as fp32 bits: ordered like unsigned integers, with infinities and NaNs on top
-__device__ __forceinline__ uint32_t mx_amax8(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return m;
-}
-
-// Quantises the eight values of this lane; the four lanes of a quad hold one block. Returns the codes and the
-// block's biased exponent (a block with an infinity or a NaN: exponent 255, codes 0).
-__device__ __forceinline__ uint32_t mx_quantize_quad(float (&v)[8], uint32_t& e) {
-  uint32_t m = mx_amax8(v);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  e = mx_exponent(m);
+// Codes of N (8 or 16) values under exponent e, N/8 words; a block with an infinity or a NaN (e = 255) gets codes 0.
+template <int N>
+__device__ __forceinline__ void mx_codes(float (&v)[N], uint32_t e, uint32_t (&q)[N / 8]) {
   const float inv = e == 255u ? 0.f : mx_inverse(e);
+  const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= inv;
-  const uint32_t c = mx_encode8(v);
-  return e == 255u ? 0u : c;
+  for (int w = 0; w < N / 8; ++w) {
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = mul_f32x2(make_float2(v[8 * w + 2 * i], v[8 * w + 2 * i + 1]), inv2);
+      s[2 * i] = f.x;
+      s[2 * i + 1] = f.y;
+    }
+    const uint32_t c = mx_encode8(s);
+    q[w] = e == 255u ? 0u : c;
+  }
 }
 
 // ------------------------------------------------------------------ 16/32-bit element types
 template <typename T> struct MxElem;
 template <> struct MxElem<__half> {
   static constexpr int kVec = 1;  // 16-byte words per eight values
+  // fp32 bits of a |value| from its 16 bits (ordered alike, infinities and NaNs on top)
+  static __device__ __forceinline__ uint32_t abs_bits(uint32_t h) {
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+  }
   static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ uint32_t put2(float a, float b) {
@@ -108,6 +111,7 @@ template <> struct MxElem<__half> {
 };
 template <> struct MxElem<__nv_bfloat16> {
   static constexpr int kVec = 1;
+  static __device__ __forceinline__ uint32_t abs_bits(uint32_t h) { return h << 16; }
   static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ uint32_t put2(float a, float b) {
@@ -124,38 +128,80 @@ template <> struct MxElem<float> {
   static __device__ __forceinline__ float put(float v) { return v; }
 };
 
+// 32 bytes of a row as loaded: 16 values of 16 bits or 8 of 32 bits
 template <typename T>
-struct MxRaw8 { uint4 w[MxElem<T>::kVec]; };  // eight elements as loaded
+struct MxRaw {
+  static constexpr int kN = 32 / sizeof(T);
+  uint32_t w[8];
+};
 
 template <typename T>
-__device__ __forceinline__ void mx_unpack8(const MxRaw8<T>& r, float (&v)[8]) {
-  if constexpr (MxElem<T>::kVec == 2) {
-    const float* f = reinterpret_cast<const float*>(r.w);
+__device__ __forceinline__ void mx_unpack(const MxRaw<T>& r, float (&v)[MxRaw<T>::kN]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = f[i];
-  } else {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = MxElem<T>::get2(w[i]);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r.w[i]);
+    } else {
+      const float2 f = MxElem<T>::get2(r.w[i]);
       v[2 * i] = f.x;
       v[2 * i + 1] = f.y;
     }
   }
 }
+
+// max |value| of the raw 32 bytes: 32-bit values as fp32 bits; 16-bit values two at a time as packed 16-bit
+// integers (half the integer instructions of widening first)
+template <typename T>
+__device__ __forceinline__ uint32_t mx_raw_amax(const MxRaw<T>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    m = sizeof(T) == 4 ? max(m, r.w[i] & 0x7FFFFFFFu) : __vmaxu2(m, r.w[i] & 0x7FFF7FFFu);
+  return m;
+}
+// ... of the whole block, over the lanes that share it (a pair of lanes of 16 values, a quad of 8), as fp32 bits
+template <typename T>
+__device__ __forceinline__ uint32_t mx_block_amax(uint32_t m) {
+  if constexpr (sizeof(T) == 4) {
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  } else {
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return MxElem<T>::abs_bits(max(m & 0xFFFFu, m >> 16));
+  }
+}
+
+__device__ __forceinline__ void mx_ld32(const void* p, uint32_t (&w)[8]) {  // 32-byte aligned
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void mx_st32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
+               : "memory");
+}
+
+// eight 16-bit values <-> fp32
+template <typename T>
+__device__ __forceinline__ void mx_unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = MxElem<T>::get2(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
 template <typename T>
 __device__ __forceinline__ void mx_store8(T* dst, const float (&v)[8]) {  // dst 16-byte aligned
-  if constexpr (MxElem<T>::kVec == 2) {
-    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint4 u;
-    u.x = MxElem<T>::put2(v[0], v[1]);
-    u.y = MxElem<T>::put2(v[2], v[3]);
-    u.z = MxElem<T>::put2(v[4], v[5]);
-    u.w = MxElem<T>::put2(v[6], v[7]);
-    *reinterpret_cast<uint4*>(dst) = u;
-  }
+  uint4 u;
+  u.x = MxElem<T>::put2(v[0], v[1]);
+  u.y = MxElem<T>::put2(v[2], v[3]);
+  u.z = MxElem<T>::put2(v[4], v[5]);
+  u.w = MxElem<T>::put2(v[6], v[7]);
+  *reinterpret_cast<uint4*>(dst) = u;
 }
 
 }  // namespace sdg

@@ -147,8 +147,8 @@ SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, in
   if (!x || !gamma || !beta || !codes || !scales || !stats_scratch || B <= 0 || HW <= 0 || C <= 0 || groups <= 0)
     return op_fail(SDG_ERR_ARG, "groupnorm_mx4: bad arguments");
   if (dtype != sdg::kF16 && dtype != sdg::kBF16) return op_fail(SDG_ERR_ARG, "groupnorm_mx4: dtype must be fp16 or bf16");
-  if (C % 8 || C % groups || C > kMaxK || B > 65535 || (int64_t)B * HW > INT32_MAX)
-    return op_fail(SDG_ERR_SHAPE, "groupnorm_mx4: C must be a multiple of 8 and of groups, B at most 65535, B * HW below 2^31");
+  if (C % 8 || C % groups || C > 4096 || B > 65535 || (int64_t)B * HW > INT32_MAX)
+    return op_fail(SDG_ERR_SHAPE, "groupnorm_mx4: C must be a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW below 2^31");
   if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(stats_scratch, 8) || !aligned(gamma, 4) ||
       !aligned(beta, 4))
     return op_fail(SDG_ERR_ARG, "groupnorm_mx4: x, codes and scales must be 16-byte aligned");

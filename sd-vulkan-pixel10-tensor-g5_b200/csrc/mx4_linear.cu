@@ -46,8 +46,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) mx4_rows_kernel(Mx4LinearArgs
     float wsc[NW];
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const uint2 q = __ldg(reinterpret_cast<const uint2*>(a.wcodes + (size_t)wr[w] * (kp / 2)) + u);
-      wsc[w] = mx_pow2(__ldg(a.wscales + ((size_t)(wr[w] >> 7) * kts + (b >> 2)) * kMxTileBytes + mx_scale_byte(wr[w], b)));
+      const uint2 q = *(reinterpret_cast<const uint2*>(a.wcodes + (size_t)wr[w] * (kp / 2)) + u);
+      wsc[w] = mx_pow2(a.wscales[((size_t)(wr[w] >> 7) * kts + (b >> 2)) * kMxTileBytes + mx_scale_byte(wr[w], b)]);
       __half2 h[4];
       mx_decode8(q.x, h);
 #pragma unroll
@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(kGThreads, 1)
             bulk_wait_read<1>();  // this buffer's previous store has read it
           }
         }
-        bias_s[lane] = p.bias && n + lane < p.N ? __ldg(p.bias + n + lane) : 0.f;
-        bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? __ldg(p.bias + n + 32 + lane) : 0.f;
+        bias_s[lane] = p.bias && n + lane < p.N ? p.bias[n + lane] : 0.f;
+        bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? p.bias[n + 32 + lane] : 0.f;
         __syncwarp();
         if (p.residual) {
           ok = mbar_wait(res_bar(w, b), (q >> 1) & 1u, p.err, kDevTimeoutEmpty);
@@ -358,10 +358,8 @@ __global__ void __launch_bounds__(kGThreads, 1)
                             __uint_as_float(r[8 * g + 4]) + b1.x, __uint_as_float(r[8 * g + 5]) + b1.y,
                             __uint_as_float(r[8 * g + 6]) + b1.z, __uint_as_float(r[8 * g + 7]) + b1.w};
               if (p.residual) {
-                MxRaw8<T> raw;
-                raw.w[0] = *reinterpret_cast<const uint4*>(at);
                 float rv[8];
-                mx_unpack8<T>(raw, rv);
+                mx_unpack8<T>(*reinterpret_cast<const uint4*>(at), rv);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] += rv[i];
               }

@@ -1,10 +1,18 @@
 // mx4_quant.cu — MXFP4 quantisation and read-back, and GroupNorm (+ SiLU) written as an MXFP4 operand.
 //
-// All three walk the operand in its own scale tiles: one block of 256 threads per 128 rows x 128 columns,
-// a half-warp per row and eight columns a lane (16-byte loads of 16-bit elements), a quad of lanes per
-// 32-column block, whose maximum is two shuffles. Every load of the tile is issued before the first use (eight
-// per thread), so a block keeps 32 KB of 16-bit input in flight. A row's codes leave as 64 contiguous bytes, the
-// tile's 512 scale bytes are gathered in shared memory and leave as one.
+// All three walk the operand in its own scale tiles: one block of 256 threads per 128 rows x 128 columns. A lane
+// takes 32 bytes of a row (16 columns of a 16-bit type, 8 of fp32), so a 32-column block is a pair (quad) of
+// lanes and its maximum one (two) shuffles, and every load of the tile is issued before the first use (32 KB of
+// 16-bit input in flight per block). A row's codes leave as 64 contiguous bytes; the tile's 512 scale bytes are
+// gathered in shared memory and leave as one. Bound by HBM: one read of x and 17/32 of a byte per value written (read
+// back: the reverse).
+//
+// Rows that 32-byte accesses cannot take (odd K, odd strides, unaligned views) go through shared memory: the warp
+// moves the row's 128 columns one element a lane, and each lane then handles its own 32 bytes of the tile.
+//
+// Inputs are read with plain loads, never through the non-coherent path (ld.global.nc, __ldg, const __restrict__): a
+// kernel launched early (programmatic launch) may share an SM's L1 with an older kernel that still reads the buffer's
+// previous contents, and only plain loads are ordered by griddepcontrol.wait.
 #include <algorithm>
 
 #include "mx4.cuh"
@@ -16,231 +24,499 @@ namespace sdg {
 namespace {
 
 constexpr int kQThreads = 256;
-constexpr int kQRows = kQThreads / 16;             // rows per pass
-constexpr int kQPass = kMxTileRows / kQRows;       // passes per tile
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_raw8(const T* src, int left, MxRaw8<T>& r) {  // left: columns from src to K
-  if constexpr (VEC) {
+// How a tile maps to threads for elements of T: kN columns a lane, kLanes lanes a row, kRows rows a pass.
+template <typename T>
+struct QMap {
+  static constexpr int kN = MxRaw<T>::kN;
+  static constexpr int kLanes = kMxTileCols / kN;
+  static constexpr int kRows = kQThreads / kLanes;
+  static constexpr int kPass = kMxTileRows / kRows;
+  static constexpr int kPitch = kMxTileCols * (int)sizeof(T) + 16;  // staged row pitch: conflict-free 16-byte reads
+};
+
+// Access widths: 32 bytes (K a multiple of the lane's columns, rows 32-byte aligned), 16 bytes, staged.
+enum Access { kW32 = 0, kW16 = 1, kStaged = 2 };
+
+// The lane's 32 bytes at src, of which `left` columns are inside the row.
+template <typename T, int ACC>
+__device__ __forceinline__ void load_raw(const T* src, int left, MxRaw<T>& r) {
+  constexpr int H = 16 / (int)sizeof(T);  // columns per 16 bytes
+  if constexpr (ACC == kW32) {
+    if (left > 0) {
+      mx_ld32(src, r.w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < MxElem<T>::kVec; ++i)
-      r.w[i] = left > 0 ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 8; ++i) r.w[i] = 0u;
+    }
   } else {
-    T* e = reinterpret_cast<T*>(r.w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < left ? src[i] : MxElem<T>::put(0.f);
+    for (int h = 0; h < 2; ++h) {
+      const uint4 u = left > h * H ? reinterpret_cast<const uint4*>(src)[h] : make_uint4(0u, 0u, 0u, 0u);
+      r.w[4 * h] = u.x; r.w[4 * h + 1] = u.y; r.w[4 * h + 2] = u.z; r.w[4 * h + 3] = u.w;
+    }
   }
 }
 
-// Writes the scale tile gathered in shared memory and zeroes it where no row or block is.
-__device__ __forceinline__ void put_scale_tile(const uint32_t* tile, uint8_t* dst) {
-  if (threadIdx.x < kMxTileBytes / 4) reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = tile[threadIdx.x];
+// The lane's codes and its block's exponent byte into the tile (c: first column of the lane, rl: row of the tile).
+template <typename T>
+__device__ __forceinline__ void put_codes(const uint32_t (&q)[QMap<T>::kN / 8], uint32_t e, int l, int rl, int c,
+                                          uint8_t* row_codes, uint32_t* tile) {
+  if constexpr (QMap<T>::kN == 16)
+    *reinterpret_cast<uint2*>(row_codes + c / 2) = make_uint2(q[0], q[1]);
+  else
+    *reinterpret_cast<uint32_t*>(row_codes + c / 2) = q[0];
+  constexpr int B = kMxBlock / QMap<T>::kN;  // lanes per block
+  if (l % B == 0) reinterpret_cast<uint8_t*>(tile)[mx_scale_byte(rl, l / B)] = (uint8_t)e;
 }
 
-// VEC: K a multiple of 8, x and its row stride 16-byte aligned.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T* __restrict__ x, int M, int K, long long ldx,
-                                                                 uint8_t* __restrict__ codes,
-                                                                 uint8_t* __restrict__ scales) {
+template <typename T, int ACC>
+__global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T* x, int M, int K, long long ldx,
+                                                                 uint8_t* codes,
+                                                                 uint8_t* scales) {
+  using Q = QMap<T>;
   __shared__ uint32_t tile[kMxTileBytes / 4];
+  extern __shared__ uint4 stage[];  // staged access only
   const int kt = blockIdx.y, kts = gridDim.y;
   const int row0 = blockIdx.x * kMxTileRows;
-  const int l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-  const int c = kt * kMxTileCols + l16 * 8;
+  const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
+  const int c = kt * kMxTileCols + l * Q::kN;
   const int kp = mx_kp(K);
   if (threadIdx.x < kMxTileBytes / 4) tile[threadIdx.x] = 0u;
   pdl_wait();
   pdl_trigger();
-  MxRaw8<T> raw[kQPass];
+  MxRaw<T> raw[Q::kPass];
+  if constexpr (ACC == kStaged) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T* st = reinterpret_cast<T*>(stage);
+    const int rows = min(kMxTileRows, M - row0);
+#pragma unroll 4
+    for (int r = warp; r < rows; r += kQThreads / 32) {
+      const T* src = x + (size_t)(row0 + r) * ldx + kt * kMxTileCols;
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int r = row0 + p * kQRows + r0;
-    load_raw8<T, VEC>(x + (size_t)min(r, M - 1) * ldx + c, r < M ? K - c : 0, raw[p]);
-  }
-  __syncthreads();
+      for (int i = 0; i < 4; ++i) {
+        const int cc = lane + 32 * i;
+        st[r * (Q::kPitch / (int)sizeof(T)) + cc] = kt * kMxTileCols + cc < K ? src[cc] : MxElem<T>::put(0.f);
+      }
+    }
+  } else {
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int rl = p * kQRows + r0, r = row0 + rl;
-    float v[8];
-    mx_unpack8<T>(raw[p], v);
-    uint32_t e;
-    const uint32_t q = mx_quantize_quad(v, e);
-    if (r < M && c < kp) {
-      *reinterpret_cast<uint32_t*>(codes + (size_t)r * (kp / 2) + c / 2) = q;
-      if ((l16 & 3) == 0) reinterpret_cast<uint8_t*>(tile)[mx_scale_byte(rl, l16 >> 2)] = (uint8_t)e;
+    for (int p = 0; p < Q::kPass; ++p) {
+      const int r = row0 + p * Q::kRows + r0;
+      load_raw<T, ACC>(x + (size_t)min(r, M - 1) * ldx + c, r < M ? K - c : 0, raw[p]);
     }
   }
   __syncthreads();
-  put_scale_tile(tile, scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes);
+#pragma unroll
+  for (int p = 0; p < Q::kPass; ++p) {
+    const int rl = p * Q::kRows + r0, r = row0 + rl;
+    if constexpr (ACC == kStaged) {
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(stage) + rl * Q::kPitch + l * 32);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 u = r < M ? src[h] : make_uint4(0u, 0u, 0u, 0u);
+        raw[p].w[4 * h] = u.x; raw[p].w[4 * h + 1] = u.y; raw[p].w[4 * h + 2] = u.z; raw[p].w[4 * h + 3] = u.w;
+      }
+    }
+    const uint32_t e = mx_exponent(mx_block_amax<T>(mx_raw_amax<T>(raw[p])));
+    float v[Q::kN];
+    mx_unpack<T>(raw[p], v);
+    uint32_t q[Q::kN / 8];
+    mx_codes<Q::kN>(v, e, q);
+    if (r < M && c < kp) put_codes<T>(q, e, l, rl, c, codes + (size_t)r * (kp / 2), tile);
+  }
+  __syncthreads();
+  if (threadIdx.x < kMxTileBytes / 4)
+    reinterpret_cast<uint32_t*>(scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x] = tile[threadIdx.x];
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                                   const uint8_t* __restrict__ scales, int M, int K,
-                                                                   T* __restrict__ y) {
+template <typename T, int ACC>
+__global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t* codes,
+                                                                   const uint8_t* scales, int M, int K,
+                                                                   T* y) {
+  using Q = QMap<T>;
   __shared__ uint32_t tile[kMxTileBytes / 4];
+  extern __shared__ uint4 stage[];  // staged access only
   const int kt = blockIdx.y, kts = gridDim.y;
   const int row0 = blockIdx.x * kMxTileRows;
-  const int l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-  const int c = kt * kMxTileCols + l16 * 8;
+  const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
+  const int c = kt * kMxTileCols + l * Q::kN;
   const int kp = mx_kp(K);
   pdl_wait();
   pdl_trigger();
   if (threadIdx.x < kMxTileBytes / 4)
     tile[threadIdx.x] =
         reinterpret_cast<const uint32_t*>(scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x];
-  uint32_t q[kQPass];
+  uint32_t q[Q::kPass][Q::kN / 8];
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int r = row0 + p * kQRows + r0;
-    q[p] = (r < M && c < kp) ? *reinterpret_cast<const uint32_t*>(codes + (size_t)r * (kp / 2) + c / 2) : 0u;
+  for (int p = 0; p < Q::kPass; ++p) {
+    const int r = row0 + p * Q::kRows + r0;
+    const bool in = r < M && c < kp;
+    const uint8_t* src = codes + (size_t)r * (kp / 2) + c / 2;
+    if constexpr (Q::kN == 16) {
+      const uint2 u = in ? *reinterpret_cast<const uint2*>(src) : make_uint2(0u, 0u);
+      q[p][0] = u.x;
+      q[p][Q::kN / 8 - 1] = u.y;
+    } else {
+      q[p][0] = in ? *reinterpret_cast<const uint32_t*>(src) : 0u;
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int rl = p * kQRows + r0, r = row0 + rl;
-    if (r >= M || c >= K) continue;
-    const float s = mx_pow2(reinterpret_cast<const uint8_t*>(tile)[mx_scale_byte(rl, l16 >> 2)]);
-    __half2 h[4];
-    mx_decode8(q[p], h);
-    float v[8];
+  for (int p = 0; p < Q::kPass; ++p) {
+    const int rl = p * Q::kRows + r0, r = row0 + rl;
+    const float s = mx_pow2(reinterpret_cast<const uint8_t*>(tile)[mx_scale_byte(rl, l / (kMxBlock / Q::kN))]);
+    uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
+    for (int w = 0; w < Q::kN / 8; ++w) {
+      __half2 h[4];
+      mx_decode8(q[p][w], h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = mul_f32x2(__half22float2(h[i]), make_float2(s, s));
+        if constexpr (sizeof(T) == 4) {
+          o[2 * i] = __float_as_uint(f.x);
+          o[2 * i + 1] = __float_as_uint(f.y);
+        } else {
+          o[4 * w + i] = MxElem<T>::put2(f.x, f.y);
+        }
+      }
     }
-    T* dst = y + (size_t)r * K + c;
-    if constexpr (VEC) {
-      mx_store8<T>(dst, v);
-    } else {
+    if constexpr (ACC == kStaged) {
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(stage) + rl * Q::kPitch + l * 32);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    } else if (r < M) {
+      T* dst = y + (size_t)r * K + c;
+      if constexpr (ACC == kW32) {
+        if (c < K) mx_st32(dst, o);
+      } else {
+        if (c < K) reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        if (c + Q::kN / 2 < K) reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    }
+  }
+  if constexpr (ACC == kStaged) {
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T* st = reinterpret_cast<const T*>(stage);
+    const int rows = min(kMxTileRows, M - row0), cols = min(kMxTileCols, K - kt * kMxTileCols);
+#pragma unroll 4
+    for (int r = warp; r < rows; r += kQThreads / 32) {
+      T* dst = y + (size_t)(row0 + r) * K + kt * kMxTileCols;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < K) dst[i] = MxElem<T>::put(v[i]);
+      for (int i = 0; i < 4; ++i) {
+        const int cc = lane + 32 * i;
+        if (cc < cols) dst[cc] = st[r * (Q::kPitch / (int)sizeof(T)) + cc];
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------ GroupNorm (+ SiLU) -> MXFP4
-__device__ __forceinline__ float gn_block_sum(float v, float* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.f;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) t += red[w];
-  __syncthreads();
-  return t;
+// Two launches. Statistics: each block reads one chunk of an image's pixels (about 32 KB, all channels) once and
+// writes each group's (mean, M2 = sum of squared differences from that mean) over the chunk. Apply: each block
+// merges the chunks' pairs of the groups its tile needs, in chunk order, then normalises, activates and quantises its
+// tile. All merges use Chan, Golub and LeVeque's update of (n, mean, M2), so no sum of squares of uncentred values is
+// ever formed, whatever a group's mean or its first pixels are. Chunks depend on (HW, C) alone: an image's result does
+// not depend on the batch, and no atomics make the order of a sum vary. The second read of x comes from L2 while an
+// input fits it.
+constexpr int kGnThreads = 256;
+constexpr int kGnBatch = 8;         // pixels a thread holds at once
+constexpr int kGnMaxC = 4096;
+constexpr int kGnMaxChunks = 128;
+constexpr int kGnTableGroups = kMxTileCols;  // groups a 128-column tile can touch (one per channel)
+
+struct GnPlan {
+  int chunk, chunks;  // pixels per chunk, chunks per image
+};
+__host__ __device__ inline int gn_rows_par(int C) { return C / 8 >= kGnThreads ? 1 : kGnThreads / (C / 8); }
+GnPlan gn_plan(int HW, int C) {
+  const int unit = gn_rows_par(C) * kGnBatch;
+  const int units = (HW + unit - 1) / unit;
+  const int per = (units + kGnMaxChunks - 1) / kGnMaxChunks;
+  GnPlan p;
+  p.chunk = per * unit;
+  p.chunks = (HW + p.chunk - 1) / p.chunk;
+  return p;
 }
 
-// One block per (group, image): mean, then the centred variance, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(512) mx4_gn_stats_kernel(const T* __restrict__ x, int HW, int C, int groups, float eps,
-                                                           float2* __restrict__ stat) {
-  __shared__ float red[16];
+__global__ void __launch_bounds__(kGnThreads) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
+                                                                  int chunk, float2* part) {
+  // (mean, M2) per thread row and channel
+  __shared__ float2 acc[kGnMaxC];
+  const int nv = C / 8, par = gn_rows_par(C), cpg = C / groups;
+  const int p0 = blockIdx.x * chunk, p1 = min(HW, p0 + chunk);
+  const int r = threadIdx.x / nv;  // thread row (0 where a row of C needs more than all threads)
   pdl_wait();
   pdl_trigger();
-  const int g = blockIdx.x, img = blockIdx.y, cpg = C / groups;
-  const T* base = x + (size_t)img * HW * C + g * cpg;
-  const long long n = (long long)HW * cpg;
-  float s = 0.f;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) s += MxElem<T>::get(base[(i / cpg) * C + i % cpg]);
-  const float mu = gn_block_sum(s, red) / (float)n;
-  float m2 = 0.f;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) {
-    const float d = MxElem<T>::get(base[(i / cpg) * C + i % cpg]) - mu;
-    m2 += d * d;
+  for (int v = threadIdx.x - (par > 1 ? r * nv : 0); v < nv; v += kGnThreads) {
+    if (par > 1 && r >= par) break;
+    const T* src = x + ((size_t)blockIdx.y * HW + p0) * C + v * 8;
+    const int first = par > 1 ? r : 0;
+    const int cnt = p1 - p0 > first ? (p1 - p0 - first + par - 1) / par : 0;  // this thread's pixels
+    float mean[8], m2[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mean[e] = m2[e] = 0.f;
+    for (int i0 = 0; i0 < cnt; i0 += kGnBatch) {
+      const int nb = min(kGnBatch, cnt - i0);
+      uint4 raw[kGnBatch];
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i)
+        raw[i] = i < nb ? *reinterpret_cast<const uint4*>(src + (size_t)(first + (i0 + i) * par) * C)
+                        : make_uint4(0u, 0u, 0u, 0u);
+      float s[8], d2[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = d2[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i) {
+        float f[8];
+        mx_unpack8<T>(raw[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += f[e];
+      }
+      const float inv = 1.f / (float)nb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] *= inv;
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i) {
+        if (i < nb) {
+          float f[8];
+          mx_unpack8<T>(raw[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float d = f[e] - s[e];
+            d2[e] = fmaf(d, d, d2[e]);
+          }
+        }
+      }
+      const float w = (float)nb / (float)(i0 + nb);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = s[e] - mean[e];
+        mean[e] = fmaf(d, w, mean[e]);
+        m2[e] += d2[e] + d * d * w * (float)i0;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[(par > 1 ? r * C : 0) + v * 8 + e] = make_float2(mean[e], m2[e]);
   }
-  const float var = gn_block_sum(m2, red) / (float)n;
-  if (threadIdx.x == 0) stat[img * groups + g] = make_float2(mu, rsqrtf(var + eps));
+  __syncthreads();
+  // one warp per group: its par x cpg pairs, thread row rr holding n_rr pixels
+  const int lane = threadIdx.x & 31;
+  const int rows = p1 - p0;
+  for (int g = threadIdx.x >> 5; g < groups; g += kGnThreads / 32) {
+    const int n = par * cpg;
+    float s = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const int rr = i / cpg;
+      const int cnt = rows > rr ? (rows - rr + par - 1) / par : 0;
+      if (cnt) s += (float)cnt * acc[rr * C + g * cpg + i - rr * cpg].x;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float mu = s / ((float)rows * cpg);
+    float m2 = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const int rr = i / cpg;
+      const int cnt = rows > rr ? (rows - rr + par - 1) / par : 0;
+      if (cnt) {
+        const float2 a = acc[rr * C + g * cpg + i - rr * cpg];
+        const float d = a.x - mu;
+        m2 += a.y + (float)cnt * d * d;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+    if (lane == 0) part[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * groups + g] = make_float2(mu, m2);
+  }
+}
+
+// (mean, rstd) of group g from the chunks' pairs at part[k * groups + g]; all lanes of the warp call it.
+__device__ __forceinline__ float2 gn_merge(const float2* part, int g, int groups, int chunks, int chunk, int HW, int cpg,
+                                           float eps) {
+  const int lane = threadIdx.x & 31;
+  float s = 0.f;
+  for (int k = lane; k < chunks; k += 32) s += (float)(min(HW, (k + 1) * chunk) - k * chunk) * part[(size_t)k * groups + g].x;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float mu = s / (float)HW;
+  float m2 = 0.f;
+  for (int k = lane; k < chunks; k += 32) {
+    const float2 a = part[(size_t)k * groups + g];
+    const float d = a.x - mu;
+    m2 += a.y + (float)(min(HW, (k + 1) * chunk) - k * chunk) * cpg * d * d;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+  return make_float2(mu, rsqrtf(m2 / ((float)HW * cpg) + eps));
 }
 
 // y * sigmoid(y) to a few fp32 ulps: the rounding to four bits comes after it, so the approximation must not move
 // values across the E2M1 midpoints more often than fp32 arithmetic does
-__device__ __forceinline__ float silu_exact(float y) { return __fdividef(y, 1.f + __expf(-y)); }
+__device__ __forceinline__ float silu_fine(float y) { return __fdividef(y, 1.f + __expf(-y)); }
 
-template <typename T>
-__global__ void __launch_bounds__(kQThreads) mx4_gn_apply_kernel(const T* __restrict__ x, int M, int HW, int C, int groups,
-                                                                 const float* __restrict__ gamma,
-                                                                 const float* __restrict__ beta, int silu,
-                                                                 const float2* __restrict__ stat,
-                                                                 uint8_t* __restrict__ codes,
-                                                                 uint8_t* __restrict__ scales) {
+struct GnApply {
+  int M, HW, C, groups, chunk, chunks;
+  float eps;
+  const float* gamma;
+  const float* beta;
+  const float2* part;
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+template <typename T, int ACC, bool SILU>
+__global__ void __launch_bounds__(kQThreads) mx4_gn_apply_kernel(const T* x, const GnApply p) {
+  using Q = QMap<T>;
+  static_assert(Q::kN == 16, "16-bit elements");
   __shared__ uint32_t tile[kMxTileBytes / 4];
+  // (mean, rstd) of the tile's images and groups when chunks are merged here: an image of more than one chunk has
+  // at least kGnBatch + 1 pixels, so a tile touches at most 128 / 9 + 2 of them
+  constexpr int kImgs = kMxTileRows / (kGnBatch + 1) + 2;
+  __shared__ float2 table[kImgs * kGnTableGroups];
   const int kt = blockIdx.y, kts = gridDim.y;
   const int row0 = blockIdx.x * kMxTileRows;
-  const int l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-  const int c = kt * kMxTileCols + l16 * 8;
-  const int kp = mx_kp(C), cpg = C / groups;
+  const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
+  const int c = kt * kMxTileCols + l * Q::kN;
+  const int kp = mx_kp(p.C), cpg = p.C / p.groups;
+  const int c_end = min(p.C, (kt + 1) * kMxTileCols);
+  const int g_lo = kt * kMxTileCols / cpg, ng = (c_end - 1) / cpg - g_lo + 1;
+  const int img0 = row0 / p.HW;
   if (threadIdx.x < kMxTileBytes / 4) tile[threadIdx.x] = 0u;
-  float ga[8], be[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    ga[i] = c < C ? __ldg(gamma + c + i) : 0.f;
-    be[i] = c < C ? __ldg(beta + c + i) : 0.f;
-  }
   pdl_wait();
   pdl_trigger();
-  MxRaw8<T> raw[kQPass];
+  MxRaw<T> raw[Q::kPass];
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int r = row0 + p * kQRows + r0;
-    load_raw8<T, true>(x + (size_t)min(r, M - 1) * C + c, r < M ? C - c : 0, raw[p]);
+  for (int i = 0; i < Q::kPass; ++i) {
+    const int r = row0 + i * Q::kRows + r0;
+    load_raw<T, ACC>(x + (size_t)min(r, p.M - 1) * p.C + c, r < p.M ? p.C - c : 0, raw[i]);
+  }
+  if (p.chunks > 1) {
+    const int imgs = (min(p.M, row0 + kMxTileRows) - 1) / p.HW - img0 + 1;
+    for (int i = threadIdx.x >> 5; i < imgs * ng; i += kQThreads / 32) {
+      const int im = i / ng, g = i - im * ng;
+      const float2 st = gn_merge(p.part + (size_t)(img0 + im) * p.chunks * p.groups, g_lo + g, p.groups, p.chunks, p.chunk,
+                                 p.HW, cpg, p.eps);
+      if ((threadIdx.x & 31) == 0) table[im * kGnTableGroups + g] = st;
+    }
   }
   __syncthreads();
+  const float inv_n = 1.f / ((float)p.HW * cpg);
+  float2 sc[8], sh[8];  // y = x * sc + sh for the lane's 16 channels of image `cur`
+  int cur = -1;
 #pragma unroll
-  for (int p = 0; p < kQPass; ++p) {
-    const int rl = p * kQRows + r0, r = row0 + rl;
-    float v[8];
-    mx_unpack8<T>(raw[p], v);
-    if (r < M && c < C) {
-      const float2* st = stat + (size_t)(r / HW) * groups;
+  for (int i = 0; i < 8; ++i) sc[i] = sh[i] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 s = st[(c + i) / cpg];
-        v[i] = (v[i] - s.x) * s.y * ga[i] + be[i];
-        if (silu) v[i] = silu_exact(v[i]);
+  for (int i = 0; i < Q::kPass; ++i) {
+    const int rl = i * Q::kRows + r0, r = row0 + rl;
+    const int img = r / p.HW;
+    if (img != cur && r < p.M && c < p.C) {
+      cur = img;
+      int g = -1;
+      float2 st = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int cc = c + j;
+        if (cc < p.C) {
+          const int gj = cc / cpg;
+          if (gj != g) {
+            g = gj;
+            if (p.chunks > 1) {
+              st = table[(img - img0) * kGnTableGroups + g - g_lo];
+            } else {
+              st = p.part[(size_t)img * p.groups + g];
+              st.y = rsqrtf(st.y * inv_n + p.eps);
+            }
+          }
+          const float a = st.y * p.gamma[cc];
+          const float b = fmaf(-st.x, a, p.beta[cc]);
+          if (j & 1) { sc[j / 2].y = a; sh[j / 2].y = b; } else { sc[j / 2].x = a; sh[j / 2].x = b; }
+        } else {
+          if (j & 1) { sc[j / 2].y = 0.f; sh[j / 2].y = 0.f; } else { sc[j / 2].x = 0.f; sh[j / 2].x = 0.f; }
+        }
       }
-    } else {
+    }
+    float v[16];
+    uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int j = 0; j < 8; ++j) {
+      float2 y = fma_f32x2(MxElem<T>::get2(raw[i].w[j]), sc[j], sh[j]);
+      if constexpr (SILU) {
+        y.x = silu_fine(y.x);
+        y.y = silu_fine(y.y);
+      }
+      v[2 * j] = y.x;
+      v[2 * j + 1] = y.y;
+      m = max(m, max(__float_as_uint(y.x) & 0x7FFFFFFFu, __float_as_uint(y.y) & 0x7FFFFFFFu));
     }
-    uint32_t e;
-    const uint32_t q = mx_quantize_quad(v, e);
-    if (r < M && c < kp) {
-      *reinterpret_cast<uint32_t*>(codes + (size_t)r * (kp / 2) + c / 2) = q;
-      if ((l16 & 3) == 0) reinterpret_cast<uint8_t*>(tile)[mx_scale_byte(rl, l16 >> 2)] = (uint8_t)e;
-    }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    const uint32_t e = mx_exponent(m);
+    uint32_t q[2];
+    mx_codes<16>(v, e, q);
+    if (r < p.M && c < kp) put_codes<T>(q, e, l, rl, c, p.codes + (size_t)r * (kp / 2), tile);
   }
   __syncthreads();
-  put_scale_tile(tile, scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes);
+  if (threadIdx.x < kMxTileBytes / 4)
+    reinterpret_cast<uint32_t*>(p.scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x] =
+        tile[threadIdx.x];
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The widest access that a row-major matrix of K columns and row stride ld allows.
+template <typename T>
+Access access_of(const T* p, int K, long long ld) {
+  const long long b = ld * (long long)sizeof(T);
+  if (K % (32 / (int)sizeof(T)) == 0 && aligned(p, 32) && b % 32 == 0) return kW32;
+  if (K % (16 / (int)sizeof(T)) == 0 && aligned(p, 16) && b % 16 == 0) return kW16;
+  return kStaged;
+}
+template <typename T>
+constexpr size_t stage_bytes() { return (size_t)kMxTileRows * QMap<T>::kPitch; }
+
+// Dynamic shared memory above 48 KB (the staged fp32 tile) is opted into once per device and kernel.
+template <typename K>
+cudaError_t allow_smem(K k, size_t bytes) {
+  return bytes > 48 * 1024 ? cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+}
 
 template <typename T>
 cudaError_t quantize_t(const T* x, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, cudaStream_t s) {
   const dim3 grid(mx_rtiles(M), mx_ktiles(K));
-  const bool vec = K % 8 == 0 && aligned16(x) && (ldx * sizeof(T)) % 16 == 0;
-  auto k = vec ? mx4_quantize_kernel<T, true> : mx4_quantize_kernel<T, false>;
-  return launch_kernel(k, grid, dim3(kQThreads), 0, s, 0, x, M, K, ldx, codes, scales);
+  const Access acc = access_of(x, K, ldx);
+  auto k = acc == kW32 ? mx4_quantize_kernel<T, kW32> : acc == kW16 ? mx4_quantize_kernel<T, kW16> : mx4_quantize_kernel<T, kStaged>;
+  const size_t sm = acc == kStaged ? stage_bytes<T>() : 0;
+  const cudaError_t e = allow_smem(k, sm);
+  return e != cudaSuccess ? e : launch_kernel(k, grid, dim3(kQThreads), sm, s, 0, x, M, K, ldx, codes, scales);
 }
 template <typename T>
 cudaError_t dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, int K, T* y, cudaStream_t s) {
   const dim3 grid(mx_rtiles(M), mx_ktiles(K));
-  const bool vec = K % 8 == 0 && aligned16(y);
-  auto k = vec ? mx4_dequantize_kernel<T, true> : mx4_dequantize_kernel<T, false>;
-  return launch_kernel(k, grid, dim3(kQThreads), 0, s, 0, codes, scales, M, K, y);
+  const Access acc = access_of(y, K, K);
+  auto k = acc == kW32   ? mx4_dequantize_kernel<T, kW32>
+           : acc == kW16 ? mx4_dequantize_kernel<T, kW16>
+                         : mx4_dequantize_kernel<T, kStaged>;
+  const size_t sm = acc == kStaged ? stage_bytes<T>() : 0;
+  const cudaError_t e = allow_smem(k, sm);
+  return e != cudaSuccess ? e : launch_kernel(k, grid, dim3(kQThreads), sm, s, 0, codes, scales, M, K, y);
 }
 template <typename T>
 cudaError_t groupnorm_t(const Mx4GroupNormArgs& a, cudaStream_t s) {
   const T* x = static_cast<const T*>(a.x);
-  float2* stat = reinterpret_cast<float2*>(a.stats);
-  cudaError_t e = launch_kernel(mx4_gn_stats_kernel<T>, dim3(a.groups, a.B), dim3(512), 0, s, 0, x, a.HW, a.C, a.groups,
-                                a.eps, stat);
+  float2* part = reinterpret_cast<float2*>(a.stats);
+  const GnPlan pl = gn_plan(a.HW, a.C);
+  cudaError_t e = launch_kernel(mx4_gn_stats_kernel<T>, dim3(pl.chunks, a.B), dim3(kGnThreads), 0, s, 0, x, a.HW, a.C,
+                                a.groups, pl.chunk, part);
   if (e != cudaSuccess) return e;
-  const int M = a.B * a.HW;
-  return launch_kernel(mx4_gn_apply_kernel<T>, dim3(mx_rtiles(M), mx_ktiles(a.C)), dim3(kQThreads), 0, s, 0, x, M, a.HW,
-                       a.C, a.groups, a.gamma, a.beta, a.silu, (const float2*)stat, a.codes, a.scales);
+  GnApply p;
+  p.M = a.B * a.HW; p.HW = a.HW; p.C = a.C; p.groups = a.groups; p.chunk = pl.chunk; p.chunks = pl.chunks;
+  p.eps = a.eps; p.gamma = a.gamma; p.beta = a.beta; p.part = part; p.codes = a.codes; p.scales = a.scales;
+  const bool w32 = access_of(x, a.C, a.C) == kW32;
+  auto k = a.silu ? (w32 ? mx4_gn_apply_kernel<T, kW32, true> : mx4_gn_apply_kernel<T, kW16, true>)
+                  : (w32 ? mx4_gn_apply_kernel<T, kW32, false> : mx4_gn_apply_kernel<T, kW16, false>);
+  return launch_kernel(k, dim3(mx_rtiles(p.M), mx_ktiles(a.C)), dim3(kQThreads), 0, s, 0, x, p);
 }
 
 }  // namespace
@@ -266,13 +542,12 @@ cudaError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
 }
 
 size_t mx4_groupnorm_scratch_bytes(int B, int HW, int C, int groups) {
-  (void)HW;
-  (void)C;
-  return (size_t)B * groups * sizeof(float2);
+  if (C % 8 || C > kGnMaxC) return 0;
+  return (size_t)B * gn_plan(HW, C).chunks * groups * sizeof(float2);
 }
 
 cudaError_t launch_mx4_groupnorm(const Mx4GroupNormArgs& a, cudaStream_t s) {
-  if (a.C % 8 || a.C % a.groups || !aligned16(a.x)) return cudaErrorInvalidValue;
+  if (a.C % 8 || a.C > kGnMaxC || a.C % a.groups || !aligned(a.x, 16)) return cudaErrorInvalidValue;
   switch (a.dtype) {
     case kF16: return groupnorm_t<__half>(a, s);
     case kBF16: return groupnorm_t<__nv_bfloat16>(a, s);
