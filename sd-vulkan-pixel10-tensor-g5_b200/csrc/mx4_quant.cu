@@ -3,7 +3,8 @@
 // All three walk the operand in its own scale tiles: one block of 256 threads per 128 rows x 128 columns. A lane
 // takes 32 bytes of a row (16 columns of a 16-bit type, 8 of fp32), so a 32-column block is a pair (quad) of
 // lanes and its maximum one (two) shuffles, and every load of the tile is issued before the first use (32 KB of
-// 16-bit input in flight per block). A row's codes leave as 64 contiguous bytes; the tile's 512 scale bytes are
+// 16-bit input in flight per block). The tiles of a row are neighbours in the grid, so the lines they share at a row
+// pitch that is no multiple of 128 bytes are still in L2 for the second of them. A row's codes leave as 64 contiguous bytes; the tile's 512 scale bytes are
 // gathered in shared memory and leave as one. Bound by HBM: one read of x and 17/32 of a byte per value written (read
 // back: the reverse).
 //
@@ -14,6 +15,7 @@
 // kernel launched early (programmatic launch) may share an SM's L1 with an older kernel that still reads the buffer's
 // previous contents, and only plain loads are ordered by griddepcontrol.wait.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx4.cuh"
 #include "sdg_kernels.h"
@@ -77,8 +79,8 @@ __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T* x, int
   using Q = QMap<T>;
   __shared__ uint32_t tile[kMxTileBytes / 4];
   extern __shared__ uint4 stage[];  // staged access only
-  const int kt = blockIdx.y, kts = gridDim.y;
-  const int row0 = blockIdx.x * kMxTileRows;
+  const int kts = mx_ktiles(K), kt = blockIdx.x % kts;
+  const int rt = blockIdx.x / kts, row0 = rt * kMxTileRows;
   const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
   const int c = kt * kMxTileCols + l * Q::kN;
   const int kp = mx_kp(K);
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T* x, int
   }
   __syncthreads();
   if (threadIdx.x < kMxTileBytes / 4)
-    reinterpret_cast<uint32_t*>(scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x] = tile[threadIdx.x];
+    reinterpret_cast<uint32_t*>(scales + ((size_t)rt * kts + kt) * kMxTileBytes)[threadIdx.x] = tile[threadIdx.x];
 }
 
 template <typename T, int ACC>
@@ -137,8 +139,8 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
   using Q = QMap<T>;
   __shared__ uint32_t tile[kMxTileBytes / 4];
   extern __shared__ uint4 stage[];  // staged access only
-  const int kt = blockIdx.y, kts = gridDim.y;
-  const int row0 = blockIdx.x * kMxTileRows;
+  const int kts = mx_ktiles(K), kt = blockIdx.x % kts;
+  const int rt = blockIdx.x / kts, row0 = rt * kMxTileRows;
   const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
   const int c = kt * kMxTileCols + l * Q::kN;
   const int kp = mx_kp(K);
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
   pdl_trigger();
   if (threadIdx.x < kMxTileBytes / 4)
     tile[threadIdx.x] =
-        reinterpret_cast<const uint32_t*>(scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x];
+        reinterpret_cast<const uint32_t*>(scales + ((size_t)rt * kts + kt) * kMxTileBytes)[threadIdx.x];
   uint32_t q[Q::kPass][Q::kN / 8];
 #pragma unroll
   for (int p = 0; p < Q::kPass; ++p) {
@@ -216,23 +218,30 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
 // ------------------------------------------------------------------ GroupNorm (+ SiLU) -> MXFP4
 // Two launches. Statistics: each block reads one chunk of an image's pixels (about 32 KB, all channels) once and
 // writes each group's (mean, M2 = sum of squared differences from that mean) over the chunk. Apply: each block
-// merges the chunks' pairs of the groups its tile needs, in chunk order, then normalises, activates and quantises its
-// tile. All merges use Chan, Golub and LeVeque's update of (n, mean, M2), so no sum of squares of uncentred values is
-// ever formed, whatever a group's mean or its first pixels are. Chunks depend on (HW, C) alone: an image's result does
+// merges the chunks' pairs of the groups its tiles need, in chunk order, then normalises, activates and quantises one to
+// four tiles of the same channels (as many as leave four blocks per SM). Threads' and chunks' pairs merge by Chan,
+// Golub and LeVeque's update of (n, mean, M2). Chunks depend on (HW, C) alone: an image's result does
 // not depend on the batch, and no atomics make the order of a sum vary. The second read of x comes from L2 while an
 // input fits it.
 constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 8;         // pixels a thread holds at once
+constexpr int kGnPixels = 16;       // pixels per thread and chunk, more where an image would need over kGnMaxChunks
 constexpr int kGnMaxC = 4096;
-constexpr int kGnMaxChunks = 128;
-constexpr int kGnTableGroups = kMxTileCols;  // groups a 128-column tile can touch (one per channel)
+constexpr int kGnMaxChunks = 256;
+
+// the larger value, NaN if either is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 struct GnPlan {
   int chunk, chunks;  // pixels per chunk, chunks per image
 };
 __host__ __device__ inline int gn_rows_par(int C) { return C / 8 >= kGnThreads ? 1 : kGnThreads / (C / 8); }
 GnPlan gn_plan(int HW, int C) {
-  const int unit = gn_rows_par(C) * kGnBatch;
+  const int unit = gn_rows_par(C) * kGnPixels;
   const int units = (HW + unit - 1) / unit;
   const int per = (units + kGnMaxChunks - 1) / kGnMaxChunks;
   GnPlan p;
@@ -241,11 +250,14 @@ GnPlan gn_plan(int HW, int C) {
   return p;
 }
 
+// A thread sums d and d^2 of its n pixels of a channel, d = x - k with k the mean of its first m = min(n, 8) pixels.
+// (k - mean)^2 <= M2 / m (Cauchy), so sum d^2 <= M2 (1 + n / m) and M2 = sum d^2 - (sum d)^2 / n loses at most the
+// factor 1 + n / m (3 at 16 pixels) to cancellation, whatever the data.
 template <typename T>
-__global__ void __launch_bounds__(kGnThreads) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
+__global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
                                                                   int chunk, float2* part) {
   // (mean, M2) per thread row and channel
-  __shared__ float2 acc[kGnMaxC];
+  __shared__ __align__(16) float2 acc[kGnMaxC];
   const int nv = C / 8, par = gn_rows_par(C), cpg = C / groups;
   const int p0 = blockIdx.x * chunk, p1 = min(HW, p0 + chunk);
   const int r = threadIdx.x / nv;  // thread row (0 where a row of C needs more than all threads)
@@ -256,76 +268,83 @@ __global__ void __launch_bounds__(kGnThreads) mx4_gn_stats_kernel(const T* x, in
     const T* src = x + ((size_t)blockIdx.y * HW + p0) * C + v * 8;
     const int first = par > 1 ? r : 0;
     const int cnt = p1 - p0 > first ? (p1 - p0 - first + par - 1) / par : 0;  // this thread's pixels
-    float mean[8], m2[8];
+    const T* at = src + (size_t)first * C;
+    const size_t step = (size_t)par * C;
+    float2 k[4], s1[4], s2[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mean[e] = m2[e] = 0.f;
+    for (int e = 0; e < 4; ++e) k[e] = s1[e] = s2[e] = make_float2(0.f, 0.f);
     for (int i0 = 0; i0 < cnt; i0 += kGnBatch) {
       const int nb = min(kGnBatch, cnt - i0);
       uint4 raw[kGnBatch];
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i)
-        raw[i] = i < nb ? *reinterpret_cast<const uint4*>(src + (size_t)(first + (i0 + i) * par) * C)
-                        : make_uint4(0u, 0u, 0u, 0u);
-      float s[8], d2[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = d2[e] = 0.f;
-#pragma unroll
       for (int i = 0; i < kGnBatch; ++i) {
-        float f[8];
-        mx_unpack8<T>(raw[i], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += f[e];
+        raw[i] = i < nb ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
+        at += step;
       }
-      const float inv = 1.f / (float)nb;
+      if (i0 == 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] *= inv;
+        for (int i = 0; i < kGnBatch; ++i) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[e] = add_f32x2(k[e], MxElem<T>::get2(w[e]));
+        }
+        const float inv = 1.f / (float)nb;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = mul_f32x2(k[e], make_float2(inv, inv));
+      }
 #pragma unroll
       for (int i = 0; i < kGnBatch; ++i) {
         if (i < nb) {
-          float f[8];
-          mx_unpack8<T>(raw[i], f);
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float d = f[e] - s[e];
-            d2[e] = fmaf(d, d, d2[e]);
+          for (int e = 0; e < 4; ++e) {
+            const float2 d = sub_f32x2(MxElem<T>::get2(w[e]), k[e]);
+            s1[e] = add_f32x2(s1[e], d);
+            s2[e] = fma_f32x2(d, d, s2[e]);
           }
         }
       }
-      const float w = (float)nb / (float)(i0 + nb);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = s[e] - mean[e];
-        mean[e] = fmaf(d, w, mean[e]);
-        m2[e] += d2[e] + d * d * w * (float)i0;
-      }
     }
+    const float inv = cnt ? 1.f / (float)cnt : 0.f;
+    float4* dst = reinterpret_cast<float4*>(acc + (par > 1 ? r * C : 0) + v * 8);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[(par > 1 ? r * C : 0) + v * 8 + e] = make_float2(mean[e], m2[e]);
+    for (int e = 0; e < 4; ++e) {
+      const float mx = s1[e].x * inv, my = s1[e].y * inv;
+      dst[e] = make_float4(k[e].x + mx, max_nan(fmaf(-mx, s1[e].x, s2[e].x), 0.f), k[e].y + my,
+                           max_nan(fmaf(-my, s1[e].y, s2[e].y), 0.f));
+    }
   }
   __syncthreads();
-  // one warp per group: its par x cpg pairs, thread row rr holding n_rr pixels
-  const int lane = threadIdx.x & 31;
   const int rows = p1 - p0;
-  for (int g = threadIdx.x >> 5; g < groups; g += kGnThreads / 32) {
-    const int n = par * cpg;
-    float s = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const int rr = i / cpg;
-      const int cnt = rows > rr ? (rows - rr + par - 1) / par : 0;
-      if (cnt) s += (float)cnt * acc[rr * C + g * cpg + i - rr * cpg].x;
+  if (par > 1) {  // per channel, the thread rows' pairs (row rr holds every par-th pixel) into row 0
+    for (int c = threadIdx.x; c < C; c += kGnThreads) {
+      float2 a = acc[c];
+      float n = (float)((rows + par - 1) / par);
+      for (int rr = 1; rr < par && rr < rows; ++rr) {
+        const float2 b = acc[rr * C + c];
+        const float nb = (float)((rows - rr + par - 1) / par), w = nb / (n + nb), d = b.x - a.x;
+        a.x = fmaf(d, w, a.x);
+        a.y += b.y + d * d * w * n;
+        n += nb;
+      }
+      acc[c] = a;
     }
+    __syncthreads();
+  }
+  // one warp per group: its cpg channels, `rows` pixels each
+  const int lane = threadIdx.x & 31;
+  const float inv_cpg = 1.f / (float)cpg;
+  for (int g = threadIdx.x >> 5; g < groups; g += kGnThreads / 32) {
+    float s = 0.f;
+    for (int i = lane; i < cpg; i += 32) s += acc[g * cpg + i].x;
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mu = s / ((float)rows * cpg);
+    const float mu = s * inv_cpg;
     float m2 = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const int rr = i / cpg;
-      const int cnt = rows > rr ? (rows - rr + par - 1) / par : 0;
-      if (cnt) {
-        const float2 a = acc[rr * C + g * cpg + i - rr * cpg];
-        const float d = a.x - mu;
-        m2 += a.y + (float)cnt * d * d;
-      }
+    for (int i = lane; i < cpg; i += 32) {
+      const float2 a = acc[g * cpg + i];
+      const float d = a.x - mu;
+      m2 += fmaf((float)rows * d, d, a.y);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
@@ -353,12 +372,24 @@ __device__ __forceinline__ float2 gn_merge(const float2* part, int g, int groups
   return make_float2(mu, rsqrtf(m2 / ((float)HW * cpg) + eps));
 }
 
-// y * sigmoid(y) to a few fp32 ulps: the rounding to four bits comes after it, so the approximation must not move
-// values across the E2M1 midpoints more often than fp32 arithmetic does
-__device__ __forceinline__ float silu_fine(float y) { return __fdividef(y, 1.f + __expf(-y)); }
+// y * sigmoid(y) of two values with one reciprocal, 1 / (a b): three MUFU instructions for two values instead of four
+// (the apply kernel would be bound by that pipe). A few fp32 ulps off: the rounding to four bits comes after it, so the
+// approximation must not move values across the E2M1 midpoints more often than fp32 arithmetic does. a and b are
+// capped at 2^63 so that their product stays finite: below y = -43.7 the result is off by up to |y| 2^-63, which is
+// nothing next to a block maximum that is not itself below 2^-40.
+__device__ __forceinline__ float2 silu_pair(float2 y) {
+  const float2 t = mul_f32x2(y, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  const float a = fminf(1.f + ex2_approx(t.x), 9.2233720e18f), b = fminf(1.f + ex2_approx(t.y), 9.2233720e18f);
+  const float r = rcp_approx(a * b);
+  return mul_f32x2(y, mul_f32x2(make_float2(r, r), make_float2(b, a)));
+}
+
+// Images that a tile of 128 rows touches at most, unless an image has kGnPixels pixels or fewer (and then one chunk)
+constexpr int kImgs = kMxTileRows / (kGnPixels + 1) + 2;
 
 struct GnApply {
   int M, HW, C, groups, chunk, chunks;
+  int tiles;  // row tiles per block
   float eps;
   const float* gamma;
   const float* beta;
@@ -367,100 +398,108 @@ struct GnApply {
   uint8_t* scales;
 };
 
-template <typename T, int ACC, bool SILU>
-__global__ void __launch_bounds__(kQThreads) mx4_gn_apply_kernel(const T* x, const GnApply p) {
+// FEW: images so small that a tile may touch more than kImgs of them; their factors come straight from the
+// statistics, in an instantiation of its own (inside the other's unrolled loop the code outgrew the instruction cache).
+template <typename T, int ACC, bool SILU, bool FEW>
+__global__ void __launch_bounds__(kQThreads, 3) mx4_gn_apply_kernel(const T* x, const GnApply p) {
   using Q = QMap<T>;
   static_assert(Q::kN == 16, "16-bit elements");
   __shared__ uint32_t tile[kMxTileBytes / 4];
-  // (mean, rstd) of the tile's images and groups when chunks are merged here: an image of more than one chunk has
-  // at least kGnBatch + 1 pixels, so a tile touches at most 128 / 9 + 2 of them
-  constexpr int kImgs = kMxTileRows / (kGnBatch + 1) + 2;
-  __shared__ float2 table[kImgs * kGnTableGroups];
-  const int kt = blockIdx.y, kts = gridDim.y;
-  const int row0 = blockIdx.x * kMxTileRows;
+  // y = x * a + b per image of the tile and channel; per pair of channels: a, a, b, b. Pair j of
+  // lane l is float4 j * 8 + l: the eight lanes of a row read 128 contiguous bytes
+  __shared__ __align__(16) float affine[kImgs * 2 * kMxTileCols];
+  __shared__ float2 table[kImgs * kMxTileCols];  // (mean, rstd) per image and group, where chunks are merged here
+  const int kts = mx_ktiles(p.C), kt = blockIdx.x % kts;
+  const int rt0 = blockIdx.x / kts * p.tiles, rt1 = min(rt0 + p.tiles, mx_rtiles(p.M));
   const int l = threadIdx.x % Q::kLanes, r0 = threadIdx.x / Q::kLanes;
   const int c = kt * kMxTileCols + l * Q::kN;
   const int kp = mx_kp(p.C), cpg = p.C / p.groups;
   const int c_end = min(p.C, (kt + 1) * kMxTileCols);
   const int g_lo = kt * kMxTileCols / cpg, ng = (c_end - 1) / cpg - g_lo + 1;
-  const int img0 = row0 / p.HW;
-  if (threadIdx.x < kMxTileBytes / 4) tile[threadIdx.x] = 0u;
+  const float inv_n = 1.f / ((float)p.HW * cpg);
+  auto one_chunk = [&](int img, int g) {
+    float2 st = p.part[(size_t)img * p.groups + g];
+    st.y = rsqrtf(st.y * inv_n + p.eps);
+    return st;
+  };
+  // a channel's factors from its group's statistics
+  auto factors = [&](int cc, float2 st) {
+    const float a = st.y * p.gamma[cc];
+    return make_float2(a, fmaf(-st.x, a, p.beta[cc]));
+  };
+  int have0 = -1, have1 = -1;  // images that `affine` holds
   pdl_wait();
   pdl_trigger();
-  MxRaw<T> raw[Q::kPass];
+#pragma unroll 1
+  for (int rt = rt0; rt < rt1; ++rt) {
+    const int row0 = rt * kMxTileRows;
+    MxRaw<T> raw[Q::kPass];
 #pragma unroll
-  for (int i = 0; i < Q::kPass; ++i) {
-    const int r = row0 + i * Q::kRows + r0;
-    load_raw<T, ACC>(x + (size_t)min(r, p.M - 1) * p.C + c, r < p.M ? p.C - c : 0, raw[i]);
-  }
-  if (p.chunks > 1) {
-    const int imgs = (min(p.M, row0 + kMxTileRows) - 1) / p.HW - img0 + 1;
-    for (int i = threadIdx.x >> 5; i < imgs * ng; i += kQThreads / 32) {
-      const int im = i / ng, g = i - im * ng;
-      const float2 st = gn_merge(p.part + (size_t)(img0 + im) * p.chunks * p.groups, g_lo + g, p.groups, p.chunks, p.chunk,
-                                 p.HW, cpg, p.eps);
-      if ((threadIdx.x & 31) == 0) table[im * kGnTableGroups + g] = st;
+    for (int i = 0; i < Q::kPass; ++i) {
+      const int r = row0 + i * Q::kRows + r0;
+      load_raw<T, ACC>(x + (size_t)min(r, p.M - 1) * p.C + c, r < p.M ? p.C - c : 0, raw[i]);
     }
-  }
-  __syncthreads();
-  const float inv_n = 1.f / ((float)p.HW * cpg);
-  float2 sc[8], sh[8];  // y = x * sc + sh for the lane's 16 channels of image `cur`
-  int cur = -1;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sc[i] = sh[i] = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < Q::kPass; ++i) {
-    const int rl = i * Q::kRows + r0, r = row0 + rl;
-    const int img = r / p.HW;
-    if (img != cur && r < p.M && c < p.C) {
-      cur = img;
-      int g = -1;
-      float2 st = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int cc = c + j;
-        if (cc < p.C) {
-          const int gj = cc / cpg;
-          if (gj != g) {
-            g = gj;
-            if (p.chunks > 1) {
-              st = table[(img - img0) * kGnTableGroups + g - g_lo];
-            } else {
-              st = p.part[(size_t)img * p.groups + g];
-              st.y = rsqrtf(st.y * inv_n + p.eps);
-            }
-          }
-          const float a = st.y * p.gamma[cc];
-          const float b = fmaf(-st.x, a, p.beta[cc]);
-          if (j & 1) { sc[j / 2].y = a; sh[j / 2].y = b; } else { sc[j / 2].x = a; sh[j / 2].x = b; }
-        } else {
-          if (j & 1) { sc[j / 2].y = 0.f; sh[j / 2].y = 0.f; } else { sc[j / 2].x = 0.f; sh[j / 2].x = 0.f; }
+    if (threadIdx.x < kMxTileBytes / 4) tile[threadIdx.x] = 0u;
+    const int img0 = row0 / p.HW, img1 = (min(p.M, row0 + kMxTileRows) - 1) / p.HW, imgs = img1 - img0 + 1;
+    if (!FEW && (img0 != have0 || img1 != have1)) {
+      have0 = img0;
+      have1 = img1;
+      if (p.chunks > 1) {
+        for (int i = threadIdx.x >> 5; i < imgs * ng; i += kQThreads / 32) {
+          const int im = i / ng, g = i - im * ng;
+          const float2 st = gn_merge(p.part + (size_t)(img0 + im) * p.chunks * p.groups, g_lo + g, p.groups, p.chunks,
+                                     p.chunk, p.HW, cpg, p.eps);
+          if ((threadIdx.x & 31) == 0) table[im * kMxTileCols + g] = st;
         }
+        __syncthreads();
+      }
+      for (int i = threadIdx.x; i < imgs * kMxTileCols; i += kQThreads) {
+        const int im = i / kMxTileCols, cl = i % kMxTileCols, cc = kt * kMxTileCols + cl;
+        float2 f = make_float2(0.f, 0.f);
+        if (cc < p.C) {
+          const int g = cc / cpg;
+          f = factors(cc, p.chunks > 1 ? table[im * kMxTileCols + g - g_lo] : one_chunk(img0 + im, g));
+        }
+        float* dst = affine + im * 2 * kMxTileCols + ((cl / 2 % 8) * 8 + cl / 16) * 4 + (cl & 1);
+        dst[0] = f.x;
+        dst[2] = f.y;
       }
     }
-    float v[16];
-    uint32_t m = 0;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float2 y = fma_f32x2(MxElem<T>::get2(raw[i].w[j]), sc[j], sh[j]);
-      if constexpr (SILU) {
-        y.x = silu_fine(y.x);
-        y.y = silu_fine(y.y);
+    for (int i = 0; i < Q::kPass; ++i) {
+      const int rl = i * Q::kRows + r0, r = row0 + rl;
+      const int img = imgs == 1 ? img0 : min(r, p.M - 1) / p.HW;
+      const float4* fac = reinterpret_cast<const float4*>(affine + (img - img0) * 2 * kMxTileCols + l * 4);
+      float v[16];
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float4 f;
+        if constexpr (FEW) {
+          const int c0 = min(c + 2 * j, p.C - 2);
+          const float2 f0 = factors(c0, one_chunk(img, c0 / cpg)), f1 = factors(c0 + 1, one_chunk(img, (c0 + 1) / cpg));
+          f = c + 2 * j < p.C ? make_float4(f0.x, f1.x, f0.y, f1.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          f = fac[8 * j];
+        }
+        float2 y = fma_f32x2(MxElem<T>::get2(raw[i].w[j]), make_float2(f.x, f.y), make_float2(f.z, f.w));
+        if constexpr (SILU) y = silu_pair(y);
+        v[2 * j] = y.x;
+        v[2 * j + 1] = y.y;
+        top = max_nan(top, max_nan(fabsf(y.x), fabsf(y.y)));
       }
-      v[2 * j] = y.x;
-      v[2 * j + 1] = y.y;
-      m = max(m, max(__float_as_uint(y.x) & 0x7FFFFFFFu, __float_as_uint(y.y) & 0x7FFFFFFFu));
+      uint32_t m = __float_as_uint(top) & 0x7FFFFFFFu;
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      const uint32_t e = mx_exponent(m);
+      uint32_t q[2];
+      mx_codes<16>(v, e, q);
+      if (r < p.M && c < kp) put_codes<T>(q, e, l, rl, c, p.codes + (size_t)r * (kp / 2), tile);
     }
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    const uint32_t e = mx_exponent(m);
-    uint32_t q[2];
-    mx_codes<16>(v, e, q);
-    if (r < p.M && c < kp) put_codes<T>(q, e, l, rl, c, p.codes + (size_t)r * (kp / 2), tile);
+    __syncthreads();
+    if (threadIdx.x < kMxTileBytes / 4)
+      reinterpret_cast<uint32_t*>(p.scales + ((size_t)rt * kts + kt) * kMxTileBytes)[threadIdx.x] = tile[threadIdx.x];
   }
-  __syncthreads();
-  if (threadIdx.x < kMxTileBytes / 4)
-    reinterpret_cast<uint32_t*>(p.scales + ((size_t)blockIdx.x * kts + kt) * kMxTileBytes)[threadIdx.x] =
-        tile[threadIdx.x];
 }
 
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -484,7 +523,7 @@ cudaError_t allow_smem(K k, size_t bytes) {
 
 template <typename T>
 cudaError_t quantize_t(const T* x, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, cudaStream_t s) {
-  const dim3 grid(mx_rtiles(M), mx_ktiles(K));
+  const dim3 grid(mx_rtiles(M) * mx_ktiles(K));
   const Access acc = access_of(x, K, ldx);
   auto k = acc == kW32 ? mx4_quantize_kernel<T, kW32> : acc == kW16 ? mx4_quantize_kernel<T, kW16> : mx4_quantize_kernel<T, kStaged>;
   const size_t sm = acc == kStaged ? stage_bytes<T>() : 0;
@@ -493,7 +532,7 @@ cudaError_t quantize_t(const T* x, int M, int K, long long ldx, uint8_t* codes, 
 }
 template <typename T>
 cudaError_t dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, int K, T* y, cudaStream_t s) {
-  const dim3 grid(mx_rtiles(M), mx_ktiles(K));
+  const dim3 grid(mx_rtiles(M) * mx_ktiles(K));
   const Access acc = access_of(y, K, K);
   auto k = acc == kW32   ? mx4_dequantize_kernel<T, kW32>
            : acc == kW16 ? mx4_dequantize_kernel<T, kW16>
@@ -514,9 +553,15 @@ cudaError_t groupnorm_t(const Mx4GroupNormArgs& a, cudaStream_t s) {
   p.M = a.B * a.HW; p.HW = a.HW; p.C = a.C; p.groups = a.groups; p.chunk = pl.chunk; p.chunks = pl.chunks;
   p.eps = a.eps; p.gamma = a.gamma; p.beta = a.beta; p.part = part; p.codes = a.codes; p.scales = a.scales;
   const bool w32 = access_of(x, a.C, a.C) == kW32;
-  auto k = a.silu ? (w32 ? mx4_gn_apply_kernel<T, kW32, true> : mx4_gn_apply_kernel<T, kW16, true>)
-                  : (w32 ? mx4_gn_apply_kernel<T, kW32, false> : mx4_gn_apply_kernel<T, kW16, false>);
-  return launch_kernel(k, dim3(mx_rtiles(p.M), mx_ktiles(a.C)), dim3(kQThreads), 0, s, 0, x, p);
+  auto pick = [&](auto few) {
+    constexpr bool F = decltype(few)::value;
+    return a.silu ? (w32 ? mx4_gn_apply_kernel<T, kW32, true, F> : mx4_gn_apply_kernel<T, kW16, true, F>)
+                  : (w32 ? mx4_gn_apply_kernel<T, kW32, false, F> : mx4_gn_apply_kernel<T, kW16, false, F>);
+  };
+  auto k = a.HW <= kGnPixels ? pick(std::true_type()) : pick(std::false_type());
+  const int rts = mx_rtiles(p.M), kts = mx_ktiles(a.C);
+  p.tiles = (int)std::max<long long>(1, std::min<long long>(4, (long long)rts * kts / (4 * num_sms())));
+  return launch_kernel(k, dim3((rts + p.tiles - 1) / p.tiles * kts), dim3(kQThreads), 0, s, 0, x, p);
 }
 
 }  // namespace
