@@ -327,7 +327,8 @@ SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M,
                            void* y, int* err_word, void* stream);
 
 /* The same with x [M, K] of type dtype (row stride ldx elements), quantised on the way into scratch
- * (sdg_linear_mx4_scratch_bytes(M, K) bytes, 16-byte aligned; its contents on entry do not matter). */
+ * (sdg_linear_mx4_scratch_bytes(M, K) bytes, 16-byte aligned; its contents on entry do not matter; a few rows
+ * need none: 0 bytes, scratch may be NULL). */
 SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales,
                              const float* bias, int N, const void* residual, int act, int dtype, void* y, void* scratch,
                              size_t scratch_bytes, int* err_word, void* stream);

@@ -462,110 +462,127 @@ def upsample_conv3x3(x, wp, bias4, out=None, workspace=None, err_word=None, stre
 # [ceil(rows/128), ceil(Kp/128), 512]; the layout is described in include/sdg.h. Every tensor of a call lives on
 # one CUDA device, which need not be the current one; the call runs on that device's current stream, or on
 # ``stream`` (a raw handle of a stream of that device).
+_torch = None
 _mx4_types: Dict[object, int] = {}
 
 
-def _mx4_dtype(dt, wide: bool = True) -> int:
-    if not _mx4_types:
+def _mx4_torch():
+    global _torch
+    if _torch is None:
         import torch
         _mx4_types.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+        _torch = torch
+    return _torch
+
+
+def _mx4_dtype(dt, wide: bool = True) -> int:
     code = _mx4_types.get(dt, 3)
     if code > (2 if wide else 1):
         raise SdgError(2, f"MXFP4 operators take fp16, bf16{' or fp32' if wide else ''} tensors, not {dt}")
     return code
 
 
-def _mx4_arg(t, name: str, dev, dtype=None, shape=None):
-    """Checks one tensor argument; returns its device pointer (None for a missing one)."""
-    if t is None:
-        return None
-    if t.device != dev or (dtype is not None and t.dtype != dtype):
-        raise SdgError(2, f"{name}: expected {dtype or t.dtype} on {dev}, got {t.dtype} on {t.device}")
-    if shape is not None and tuple(t.shape) != shape:
+def _mx4_arg(t, name: str, dev: int, dtype, shape) -> int:
+    """The device pointer of a tensor argument that is what it has to be."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise SdgError(2, f"{name}: expected {dtype} on cuda:{dev}, got {t.dtype} on {t.device}")
+    if t.shape != shape:
         raise SdgError(3, f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
-    if not t.is_contiguous():
-        raise SdgError(2, f"{name} must be contiguous")
-    return t.data_ptr()
+    raise SdgError(2, f"{name} must be contiguous")
 
 
-def _mx4_device(t):
-    if not t.is_cuda:
+def _mx4_device(t) -> int:
+    dev = t.get_device()
+    if dev < 0:
         raise SdgError(2, "MXFP4 operators take CUDA tensors")
-    return t.device
+    return dev
 
 
 def _mx4_scale_shape(rows: int, half: int):
     return ((rows + 127) // 128, (half + 63) // 64, 512)
 
 
-def _mx4_call(fn, dev, stream, fresh, *args) -> None:
-    """Runs one C entry on ``dev``; ``fresh``: tensors allocated by this call (from the current stream's pool),
-    which must not be reused before the work on another ``stream`` is done."""
-    import torch
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return _mx4_call(fn, dev, stream, fresh, *args)
-    if stream is None:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index) or None))
-        return
-    try:
-        check(fn(*args, stream or None))
-    finally:
-        side = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
-        for t in fresh:
-            t.record_stream(side)
+def _mx4_call(fn, dev: int, *args) -> None:
+    """Runs one C entry on the current stream of device ``dev``."""
+    T = _torch
+    if T._C._cuda_getDevice() != dev:
+        with T.cuda.device(dev):
+            return _mx4_call(fn, dev, *args)
+    code = fn(*args, T._C._cuda_getCurrentRawStream(dev))
+    if code:
+        raise SdgError(code, last_error())
 
 
-def _mx4_empty(rows: int, half: int, dev):
-    import torch
-    return (torch.empty((rows, half), dtype=torch.uint8, device=dev),
-            torch.empty(_mx4_scale_shape(rows, half), dtype=torch.uint8, device=dev))
+def _mx4_on(stream: int, like, call):
+    """``call()`` with the stream of a raw handle current: what it allocates belongs to that stream, so neither its
+    scratch nor its results can be memory that work of another stream still uses."""
+    T = _mx4_torch()
+    dev = _mx4_device(like)
+    side = T.cuda.ExternalStream(stream, device=dev) if stream else T.cuda.default_stream(dev)
+    with T.cuda.stream(side):
+        return call()
 
 
 def _mx4_rows(x):
     """(rows, K, row stride) of a 2-D tensor whose rows are contiguous."""
-    if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 1:
+    if x.dim() != 2 or x.numel() == 0:
         raise SdgError(3, f"expected a matrix with at least one row and column, got {list(x.shape)}")
     R, K = x.shape
-    if K > 1 and x.stride(1) != 1:
+    ldx, one = x.stride()
+    if one != 1 and K > 1:
         raise SdgError(2, "the columns of a row must be contiguous")
-    return R, K, x.stride(0) if R > 1 else K
+    return R, K, ldx if R > 1 else K
+
+
+def _mx4_operand(out, rows: int, half: int, like, dev: int):
+    """The (codes, scales) pair to write into, with both pointers."""
+    U8 = _torch.uint8
+    if out is None:
+        codes = like.new_empty((rows, half), dtype=U8)
+        scales = like.new_empty(_mx4_scale_shape(rows, half), dtype=U8)
+        return codes, scales, codes.data_ptr(), scales.data_ptr()
+    codes, scales = out
+    return (codes, scales, _mx4_arg(codes, "codes", dev, U8, (rows, half)),
+            _mx4_arg(scales, "scales", dev, U8, _mx4_scale_shape(rows, half)))
 
 
 def quantize_mx4(x, out=None, stream=None):
     """x [rows, K] fp16 / bf16 / fp32 (rows may be strided) -> (codes, scales) in MXFP4. ``out``: the pair to
     write into. Weights [N, K] and activations [M, K] are quantised alike."""
-    import torch
+    if stream is not None:
+        return _mx4_on(stream, x, lambda: quantize_mx4(x, out))
+    _mx4_torch()
     dev = _mx4_device(x)
     dt = _mx4_dtype(x.dtype)
     R, K, ldx = _mx4_rows(x)
-    half = (K + 31) // 32 * 16
-    codes, scales = out if out is not None else _mx4_empty(R, half, dev)
-    pc = _mx4_arg(codes, "codes", dev, torch.uint8, (R, half))
-    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(R, half))
-    _mx4_call(lib().sdg_quantize_mx4, dev, stream, () if out is not None else (codes, scales), x.data_ptr(), dt, R, K,
-              ldx, pc, ps)
+    codes, scales, pc, ps = _mx4_operand(out, R, (K + 31) // 32 * 16, x, dev)
+    _mx4_call(lib().sdg_quantize_mx4, dev, x.data_ptr(), dt, R, K, ldx, pc, ps)
     return codes, scales
 
 
 def dequantize_mx4(codes, scales, K: Optional[int] = None, dtype=None, out=None, stream=None):
     """The values an MXFP4 operand stands for, [rows, K] (all Kp columns when K is None), as ``dtype`` (fp16)."""
-    import torch
+    if stream is not None:
+        return _mx4_on(stream, codes, lambda: dequantize_mx4(codes, scales, K, dtype, out))
+    T = _mx4_torch()
     dev = _mx4_device(codes)
-    if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] < 16 or codes.shape[1] % 16:
+    if codes.dim() != 2 or codes.numel() == 0 or codes.shape[1] % 16:
         raise SdgError(3, f"codes: expected [rows, Kp/2], got {list(codes.shape)}")
     R, half = codes.shape
-    K = 2 * half if K is None else K
-    if not 2 * half - 32 < K <= 2 * half:
+    if K is None:
+        K = 2 * half
+    elif not 2 * half - 32 < K <= 2 * half:
         raise SdgError(3, f"K = {K} does not fit codes of {2 * half} columns")
-    pc = _mx4_arg(codes, "codes", dev, torch.uint8)
-    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(R, half))
-    fresh = ()
+    pc = _mx4_arg(codes, "codes", dev, T.uint8, (R, half))
+    ps = _mx4_arg(scales, "scales", dev, T.uint8, _mx4_scale_shape(R, half))
     if out is None:
-        out = torch.empty((R, K), dtype=dtype or torch.float16, device=dev)
-        fresh = (out,)
-    py = _mx4_arg(out, "out", dev, dtype, (R, K))
-    _mx4_call(lib().sdg_dequantize_mx4, dev, stream, fresh, pc, ps, R, K, _mx4_dtype(out.dtype), py)
+        out = codes.new_empty((R, K), dtype=dtype or T.float16)
+        py = out.data_ptr()
+    else:
+        py = _mx4_arg(out, "out", dev, dtype or out.dtype, (R, K))
+    _mx4_call(lib().sdg_dequantize_mx4, dev, pc, ps, R, K, _mx4_dtype(out.dtype), py)
     return out
 
 
@@ -575,77 +592,73 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
     fp16 / bf16 (quantised on the way; y has its type), or the codes [M, Kp/2] of an operand whose scales are
     ``xscale`` (y has ``dtype``, fp16 by default). w: ``quantize_mx4`` of the [N, K] weight; act 2 = GEGLU on rows
     packed by ``pack_geglu_weight`` before quantising, y [M, N/2]. ``out`` may be the residual."""
-    import torch
+    if stream is not None:
+        return _mx4_on(stream, x, lambda: linear_mx4(x, wcodes, wscales, bias, residual, act, xscale, dtype, out, err_word))
+    T = _mx4_torch()
+    U8 = T.uint8
     dev = _mx4_device(x)
-    if wcodes.dim() != 2:
-        raise SdgError(3, f"wcodes: expected [N, Kp/2], got {list(wcodes.shape)}")
-    N, half = wcodes.shape
     if xscale is None:
         M, K, ldx = _mx4_rows(x)
+        half = (K + 31) // 32 * 16
         dt = x.dtype
-        if dtype is not None and dtype != dt:
+        if dtype is not None and dtype is not dt:
             raise SdgError(2, f"y has the type of x, {dt}")
-        if half != (K + 31) // 32 * 16:
-            raise SdgError(3, f"x has {K} columns, the weight {2 * half}")
     else:
-        if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] != half or half % 16:
-            raise SdgError(3, f"x codes: expected [M, {half}], got {list(x.shape)}")
-        M, K = x.shape[0], 2 * half
-        dt = dtype or torch.float16
+        if x.dim() != 2 or x.numel() == 0 or x.shape[1] % 16:
+            raise SdgError(3, f"x codes: expected [M, Kp/2], got {list(x.shape)}")
+        M, half = x.shape
+        K = 2 * half
+        dt = dtype or T.float16
     code = _mx4_dtype(dt, wide=False)
-    pw = _mx4_arg(wcodes, "wcodes", dev, torch.uint8)
-    pws = _mx4_arg(wscales, "wscales", dev, torch.uint8, _mx4_scale_shape(N, half))
-    pb = _mx4_arg(bias, "bias", dev, torch.float32, (N,))
-    pr = _mx4_arg(residual, "residual", dev, dt, (M, N))
-    pe = _mx4_arg(err_word, "err_word", dev, torch.int32)
-    fresh = []
+    N = wcodes.shape[0] if wcodes.dim() == 2 else 0
+    pw = _mx4_arg(wcodes, "wcodes", dev, U8, (N, half))
+    pws = _mx4_arg(wscales, "wscales", dev, U8, _mx4_scale_shape(N, half))
+    pb = None if bias is None else _mx4_arg(bias, "bias", dev, T.float32, (N,))
+    pr = None if residual is None else _mx4_arg(residual, "residual", dev, dt, (M, N))
+    pe = None if err_word is None else _mx4_arg(err_word, "err_word", dev, T.int32, err_word.shape)
+    shape = (M, N // 2 if act == 2 else N)
     if out is None:
-        out = torch.empty((M, N // 2 if act == 2 else N), dtype=dt, device=dev)
-        fresh.append(out)
+        out = x.new_empty(shape, dtype=dt)
         py = out.data_ptr()
     else:
-        py = _mx4_arg(out, "out", dev, dt, (M, N // 2 if act == 2 else N))
+        py = _mx4_arg(out, "out", dev, dt, shape)
     if xscale is None:
-        nb = (M * half + 511) // 512 * 512 + ((M + 127) // 128) * ((half + 63) // 64) * 512
-        scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
-        fresh.append(scratch)
-        _mx4_call(lib().sdg_linear_mx4_x, dev, stream, fresh, x.data_ptr(), M, K, ldx, pw, pws, pb, N, pr, act, code, py,
-                  scratch.data_ptr(), nb, pe)
+        ps, nb = None, lib().sdg_linear_mx4_scratch_bytes(M, K)
+        if nb:
+            scratch = x.new_empty((nb,), dtype=U8)
+            ps = scratch.data_ptr()
+        _mx4_call(lib().sdg_linear_mx4_x, dev, x.data_ptr(), M, K, ldx, pw, pws, pb, N, pr, act, code, py,
+                  ps, nb, pe)
     else:
-        px = _mx4_arg(x, "x codes", dev, torch.uint8)
-        pxs = _mx4_arg(xscale, "xscale", dev, torch.uint8, _mx4_scale_shape(M, half))
-        _mx4_call(lib().sdg_linear_mx4, dev, stream, fresh, px, pxs, M, K, pw, pws, pb, N, pr, act, code, py, pe)
+        px = _mx4_arg(x, "x codes", dev, U8, (M, half))
+        pxs = _mx4_arg(xscale, "xscale", dev, U8, _mx4_scale_shape(M, half))
+        _mx4_call(lib().sdg_linear_mx4, dev, px, pxs, M, K, pw, pws, pb, N, pr, act, code, py, pe)
     return out
 
 
 def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=None, stats=None, stream=None):
     """GroupNorm (+ SiLU) of channels-last x [B, HW, C] fp16 / bf16, quantised as it is written: the MXFP4 operand
     (codes, scales) of the matrix [B * HW, C]. ``out``: the pair to write into."""
-    import torch
+    if stream is not None:
+        return _mx4_on(stream, x, lambda: groupnorm_mx4(x, gamma, beta, eps, silu, groups, out, stats))
+    T = _mx4_torch()
     dev = _mx4_device(x)
-    if x.dim() != 3 or 0 in x.shape:
+    if x.dim() != 3 or x.numel() == 0:
         raise SdgError(3, f"x: expected [B, HW, C], got {list(x.shape)}")
     B, HW, C = x.shape
     dt = _mx4_dtype(x.dtype, wide=False)
-    px = _mx4_arg(x, "x", dev)
-    pg = _mx4_arg(gamma, "gamma", dev, torch.float32, (C,))
-    pb = _mx4_arg(beta, "beta", dev, torch.float32, (C,))
-    half = (C + 31) // 32 * 16
-    fresh = []
-    if out is None:
-        out = _mx4_empty(B * HW, half, dev)
-        fresh += out
-    codes, scales = out
-    pc = _mx4_arg(codes, "codes", dev, torch.uint8, (B * HW, half))
-    ps = _mx4_arg(scales, "scales", dev, torch.uint8, _mx4_scale_shape(B * HW, half))
+    px = _mx4_arg(x, "x", dev, x.dtype, (B, HW, C))
+    pg = _mx4_arg(gamma, "gamma", dev, T.float32, (C,))
+    pb = _mx4_arg(beta, "beta", dev, T.float32, (C,))
+    codes, scales, pc, ps = _mx4_operand(out, B * HW, (C + 31) // 32 * 16, x, dev)
     need = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups)
     if stats is None:
-        stats = torch.empty((need // 4 + 1,), dtype=torch.float32, device=dev)
-        fresh.append(stats)
-    pt = _mx4_arg(stats, "stats", dev, torch.float32)
+        stats = x.new_empty((need // 4 + 1,), dtype=T.float32)
+    pt = _mx4_arg(stats, "stats", dev, T.float32, stats.shape)
     if stats.numel() * 4 < need:
         raise SdgError(2, f"stats: {need} bytes are needed")
-    _mx4_call(lib().sdg_groupnorm_mx4, dev, stream, fresh, px, dt, B, HW, C, groups, pg, pb, eps, int(silu), pc, ps, pt)
+    _mx4_call(lib().sdg_groupnorm_mx4, dev, px, dt, B, HW, C, groups, pg, pb, eps,
+              int(silu), pc, ps, pt)
     return codes, scales
 
 

@@ -61,15 +61,16 @@ int linear_check(const char* what, int M, int K, const uint8_t* wcodes, const ui
   return SDG_OK;
 }
 
-int linear_run(const char* what, const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
-               const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype, void* y,
-               int* err_word, cudaStream_t s) {
-  sdg::Mx4LinearArgs a;
-  a.xcodes = xcodes; a.xscales = xscales; a.wcodes = wcodes; a.wscales = wscales;
+// The codes' part of the scratch, rounded up so that the scales behind it are aligned.
+size_t code_space(int M, int K) { return ((size_t)M * (sdg::mx_kp(K) / 2) + 511) / 512 * 512; }
+
+int linear_run(sdg::Mx4LinearArgs a, int M, int K, const uint8_t* wcodes, const uint8_t* wscales, const float* bias, int N,
+               const void* residual, int act, int dtype, void* y, int* err_word, cudaStream_t s) {
+  a.wcodes = wcodes; a.wscales = wscales;
   a.M = M; a.N = N; a.K = K; a.bias = bias; a.residual = residual; a.act = act; a.dtype = dtype; a.y = y;
   int* err = err_word ? err_word : default_err_word();
-  if (!err) return op_fail(SDG_ERR_CUDA, std::string(what) + ": no device error word");
-  return status(sdg::launch_mx4_linear(a, err, s), what);
+  if (!err) return op_fail(SDG_ERR_CUDA, "linear_mx4: no device error word");
+  return status(sdg::launch_mx4_linear(a, err, s), "linear_mx4");
 }
 
 }  // namespace
@@ -113,7 +114,10 @@ SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M,
   if (st) return st;
   if (!xcodes || !xscales || !aligned(xcodes, 16) || !aligned(xscales, 16))
     return op_fail(SDG_ERR_ARG, "linear_mx4: x codes and scales must be 16-byte aligned device pointers");
-  return linear_run("linear_mx4", xcodes, xscales, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word,
+  sdg::Mx4LinearArgs a;
+  a.xcodes = xcodes;
+  a.xscales = xscales;
+  return linear_run(a, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word,
                     static_cast<cudaStream_t>(stream));
 }
 
@@ -122,18 +126,29 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
                              size_t scratch_bytes, int* err_word, void* stream) {
   int st = linear_check("linear_mx4", M, K, wcodes, wscales, bias, N, residual, act, dtype, y);
   if (st) return st;
-  const size_t cb = (sdg_mx4_code_bytes(M, K) + 511) / 512 * 512;
-  if (!x || ldx < 0 || !scratch || !aligned(scratch, 16) || !aligned(x, 2) || scratch_bytes < cb + sdg_mx4_scale_bytes(M, K))
+  const bool rows = sdg::mx4_linear_rows(M, K);
+  const size_t need = sdg_linear_mx4_scratch_bytes(M, K);
+  if (!x || ldx < 0 || !aligned(x, 2) || (need && (!scratch || !aligned(scratch, 16) || scratch_bytes < need)))
     return op_fail(SDG_ERR_ARG, "linear_mx4: bad x, or scratch smaller than sdg_linear_mx4_scratch_bytes");
-  uint8_t* xc = static_cast<uint8_t*>(scratch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = status(sdg::launch_mx4_quantize(x, dtype, M, K, ldx, xc, xc + cb, s), "linear_mx4");
-  if (st) return st;
-  return linear_run("linear_mx4", xc, xc + cb, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word, s);
+  sdg::Mx4LinearArgs a;
+  if (rows) {
+    a.x = x;
+    a.ldx = ldx;
+  } else {
+    uint8_t* xc = static_cast<uint8_t*>(scratch);
+    uint8_t* xs = xc + code_space(M, K);
+    st = status(sdg::launch_mx4_quantize(x, dtype, M, K, ldx, xc, xs, s), "linear_mx4");
+    if (st) return st;
+    a.xcodes = xc;
+    a.xscales = xs;
+  }
+  return linear_run(a, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word, s);
 }
 
 SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K) {
-  return (sdg_mx4_code_bytes(M, K) + 511) / 512 * 512 + sdg_mx4_scale_bytes(M, K);
+  if (M <= 0 || K <= 0 || K > kMaxK || sdg::mx4_linear_rows(M, K)) return 0;
+  return code_space(M, K) + sdg_mx4_scale_bytes(M, K);
 }
 
 SDG_API size_t sdg_groupnorm_mx4_scratch_bytes(int B, int HW, int C, int groups) {

@@ -1,9 +1,11 @@
 // mx4_linear.cu — y = act(x w^T + bias + residual) of two MXFP4 operands (format: mx4.cuh).
 //
-// mx4_rows_kernel: the product on the CUDA cores, one warp per output column (value and gate column for GEGLU)
-// and up to MB rows. A lane takes 16 columns at a time (8 bytes of each operand): the codes decode to fp16
-// exactly, and the eight products a half of each pair adds up stay exact in fp16 (at most 8 * 36 = 288 in steps of
-// 1/4: 1152 steps, fewer than the 2048 an fp16 significand holds). Block scales, and the sums over blocks, are fp32.
+// mx4_rows_kernel: up to eight rows (time embeddings, single tokens), on the CUDA cores: one warp per output column
+// (value and gate column for GEGLU) for all rows. A lane takes 16 columns at a time (8 bytes of each operand): the
+// codes decode to fp16 exactly, and the eight products a half of each pair adds up stay exact in fp16 (at most 8 * 36 =
+// 288 in steps of 1/4: 1152 steps, fewer than the 2048 an fp16 significand holds). Block scales, and the sums over
+// blocks, are fp32. A plain x is quantised by every block itself, so that the whole call is one launch: it is bound by
+// launch latency and one pass over the weights.
 #include <algorithm>
 #include <atomic>
 
@@ -17,77 +19,163 @@ namespace sdg {
 namespace {
 
 constexpr int kRowsWarps = 8;
+constexpr int kRowsThreads = 32 * kRowsWarps;
 
 // y * sigmoid(y), a few fp32 ulps
 __device__ __forceinline__ float silu_fine(float y) { return __fdividef(y, 1.f + __expf(-y)); }
 
-template <typename T, int MB, bool GEGLU>
-__global__ void __launch_bounds__(32 * kRowsWarps) mx4_rows_kernel(Mx4LinearArgs a) {
+// x gelu(x) factor: gelu of two values, x Phi(x) with erf from Abramowitz & Stegun 7.1.26 as in gelu_as, written as
+// max(x, 0) - |x| q with q = poly(t) exp(-x^2 / 2) / 2 = 1 - Phi(|x|), so that both signs share it without
+// cancellation; in f32x2 arithmetic with one reciprocal for both values (three MUFU instructions a pair). |x| is
+// capped at 128 where q is long zero, which keeps the product of the denominators and infinite x finite.
+__device__ __forceinline__ float2 gelu_pair(float2 x) {
+  const float2 a = make_float2(fminf(fabsf(x.x), 128.f), fminf(fabsf(x.y), 128.f));
+  const float2 den = fma_f32x2(a, make_float2(0.23164189f, 0.23164189f), make_float2(1.f, 1.f));  // p / sqrt(2)
+  const float r = rcp_approx(den.x * den.y);
+  const float2 t = mul_f32x2(make_float2(r, r), make_float2(den.y, den.x));
+  auto c2 = [](float c) { return make_float2(c, c); };
+  float2 q = fma_f32x2(t, c2(0.5f * 1.061405429f), c2(0.5f * -1.453152027f));
+  q = fma_f32x2(q, t, c2(0.5f * 1.421413741f));
+  q = fma_f32x2(q, t, c2(0.5f * -0.284496736f));
+  q = fma_f32x2(q, t, c2(0.5f * 0.254829592f));
+  q = mul_f32x2(q, t);
+  const float2 e = mul_f32x2(mul_f32x2(x, x), c2(-0.72134752f));  // -x^2 / 2 log2(e)
+  q = mul_f32x2(q, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
+  return fma_f32x2(make_float2(-a.x, -a.y), q, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+
+// a.x set (QUANT): the block quantises its rows of x itself, once, into shared memory; else it copies the operand there.
+template <typename T, int MB, bool GEGLU, bool QUANT>
+__global__ void __launch_bounds__(kRowsThreads) mx4_rows_kernel(Mx4LinearArgs a) {
+  extern __shared__ __align__(16) uint8_t rows_smem[];
+  constexpr int NW = GEGLU ? 2 : 1;
   const int lane = threadIdx.x & 31;
   const int nout = GEGLU ? a.N / 2 : a.N;
-  const int n = blockIdx.x * kRowsWarps + (threadIdx.x >> 5);
-  const int m0 = blockIdx.y * MB;
-  pdl_wait();
-  pdl_trigger();
-  if (n >= nout) return;
-  constexpr int NW = GEGLU ? 2 : 1;
-  const int kp = mx_kp(a.K), kts = mx_ktiles(a.K);
+  const int n = min((int)(blockIdx.x * kRowsWarps + (threadIdx.x >> 5)), nout - 1);
+  const bool live = blockIdx.x * kRowsWarps + (threadIdx.x >> 5) < nout;
+  const int kp = mx_kp(a.K), kts = mx_ktiles(a.K), units = kp / 16;
+  const int rows = min(MB, a.M);
+  uint8_t* xc = rows_smem;                                          // [MB][kp / 2] codes
+  float* xs = reinterpret_cast<float*>(rows_smem + MB * (kp / 2));  // [MB][kp / 32] scales
   int wr[NW];  // weight rows: GEGLU interleaves 16 value rows and their 16 gate rows
   wr[0] = GEGLU ? (n >> 4) * 32 + (n & 15) : n;
   if (GEGLU) wr[NW - 1] = wr[0] + 16;
+  pdl_wait();
+  pdl_trigger();
+  // this lane's first weights, in flight while x is quantised
+  constexpr int PRE = 4;
+  uint2 wq[NW][PRE];
+  uint32_t we[NW][PRE];
+  auto load_w = [&](int u0) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int i = 0; i < PRE; ++i) {
+        const int u = u0 + 32 * i, b = u >> 1;
+        wq[w][i] = make_uint2(0u, 0u);
+        we[w][i] = 0;
+        if (u < units) {
+          wq[w][i] = *(reinterpret_cast<const uint2*>(a.wcodes + (size_t)wr[w] * (kp / 2)) + u);
+          we[w][i] = a.wscales[((size_t)(wr[w] >> 7) * kts + (b >> 2)) * kMxTileBytes + mx_scale_byte(wr[w], b)];
+        }
+      }
+  };
+  load_w(lane);
+  if constexpr (QUANT) {
+    const T* x = static_cast<const T*>(a.x);
+    const bool vec = a.K % 8 == 0 && (a.ldx * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const int per = kp / 8, total = rows * per;  // units of eight columns; a quad of lanes holds one block
+    for (int i0 = 0; i0 < total; i0 += kRowsThreads) {
+      const int i = i0 + threadIdx.x, r = min(i / per, rows - 1), c = (i - r * per) * 8;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (i < total) {
+        const T* src = x + (size_t)r * a.ldx + c;
+        if (vec) {
+          if (c < a.K) mx_unpack8<T>(*reinterpret_cast<const uint4*>(src), v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < a.K) v[e] = MxElem<T>::get(src[e]);
+        }
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t e = mx_exponent(m);
+      uint32_t q[1];
+      mx_codes<8>(v, e, q);
+      if (i < total) {
+        *reinterpret_cast<uint32_t*>(xc + r * (kp / 2) + c / 2) = q[0];
+        if ((i & 3) == 0) xs[r * (kp / 32) + c / 32] = mx_pow2(e);
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * (kp / 32); i += kRowsThreads) {
+      const int r = i / (kp / 32), b = i - r * (kp / 32);
+      reinterpret_cast<uint4*>(xc)[i] = reinterpret_cast<const uint4*>(a.xcodes)[i];
+      xs[i] = mx_pow2(a.xscales[(size_t)(b >> 2) * kMxTileBytes + mx_scale_byte(r, b)]);
+    }
+  }
+  __syncthreads();
   float acc[NW][MB];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[w][i] = 0.f;
-  for (int u = lane; u < kp / 16; u += 32) {
-    const int b = u >> 1;
-    __half2 wv[NW][8];
-    float wsc[NW];
+  for (int u0 = lane; u0 < units; u0 += 32 * PRE) {
+    if (u0 != lane) load_w(u0);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const uint2 q = *(reinterpret_cast<const uint2*>(a.wcodes + (size_t)wr[w] * (kp / 2)) + u);
-      wsc[w] = mx_pow2(a.wscales[((size_t)(wr[w] >> 7) * kts + (b >> 2)) * kMxTileBytes + mx_scale_byte(wr[w], b)]);
-      __half2 h[4];
-      mx_decode8(q.x, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) wv[w][i] = h[i];
-      mx_decode8(q.y, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) wv[w][4 + i] = h[i];
-    }
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const int m = m0 + i;
-      if (m >= a.M) break;
-      const uint2 q = *(reinterpret_cast<const uint2*>(a.xcodes + (size_t)m * (kp / 2)) + u);
-      const float xsc = mx_pow2(a.xscales[((size_t)(m >> 7) * kts + (b >> 2)) * kMxTileBytes + mx_scale_byte(m, b)]);
-      __half2 h0[4], h1[4];
-      mx_decode8(q.x, h0);
-      mx_decode8(q.y, h1);
+    for (int i = 0; i < PRE; ++i) {
+      const int u = u0 + 32 * i;
+      if (u >= units) break;
+      __half2 wv[NW][8];
+      float wsc[NW];
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        __half2 s = __hmul2(h0[0], wv[w][0]);
+        wsc[w] = mx_pow2(we[w][i]);
+        __half2 h[4];
+        mx_decode8(wq[w][i].x, h);
 #pragma unroll
-        for (int j = 1; j < 4; ++j) s = __hfma2(h0[j], wv[w][j], s);
+        for (int j = 0; j < 4; ++j) wv[w][j] = h[j];
+        mx_decode8(wq[w][i].y, h);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s = __hfma2(h1[j], wv[w][4 + j], s);
-        const float2 f = __half22float2(s);
-        acc[w][i] += (f.x + f.y) * xsc * wsc[w];
+        for (int j = 0; j < 4; ++j) wv[w][4 + j] = h[j];
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        if (m >= rows) break;
+        const uint2 q = *(reinterpret_cast<const uint2*>(xc + m * (kp / 2)) + u);
+        const float xsc = xs[m * (kp / 32) + (u >> 1)];
+        __half2 h0[4], h1[4];
+        mx_decode8(q.x, h0);
+        mx_decode8(q.y, h1);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          __half2 s = __hmul2(h0[0], wv[w][0]);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) s = __hfma2(h0[j], wv[w][j], s);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s = __hfma2(h1[j], wv[w][4 + j], s);
+          const float2 f = __half22float2(s);
+          acc[w][m] += (f.x + f.y) * xsc * wsc[w];
+        }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
+  for (int m = 0; m < MB; ++m) {
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int o = 16; o; o >>= 1) acc[w][i] += __shfl_xor_sync(0xffffffffu, acc[w][i], o);
-    const int m = m0 + i;
-    if (lane == i && m < a.M) {
-      float v = acc[0][i] + (a.bias ? a.bias[wr[0]] : 0.f);
+      for (int o = 16; o; o >>= 1) acc[w][m] += __shfl_xor_sync(0xffffffffu, acc[w][m], o);
+    if (lane == m && m < rows && live) {
+      float v = acc[0][m] + (a.bias ? a.bias[wr[0]] : 0.f);
       if (GEGLU) {
-        v *= gelu_as(acc[NW - 1][i] + (a.bias ? a.bias[wr[NW - 1]] : 0.f));
+        v *= gelu_as(acc[NW - 1][m] + (a.bias ? a.bias[wr[NW - 1]] : 0.f));
       } else {
         if (a.residual) v += MxElem<T>::get(static_cast<const T*>(a.residual)[(size_t)m * a.N + n]);
         if (a.act == 1) v = silu_fine(v);
@@ -99,10 +187,12 @@ __global__ void __launch_bounds__(32 * kRowsWarps) mx4_rows_kernel(Mx4LinearArgs
 
 template <typename T, int MB>
 cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
-  const int nout = a.act == 2 ? a.N / 2 : a.N;
-  const dim3 grid((nout + kRowsWarps - 1) / kRowsWarps, (a.M + MB - 1) / MB);
-  auto k = a.act == 2 ? mx4_rows_kernel<T, MB, true> : mx4_rows_kernel<T, MB, false>;
-  return launch_kernel(k, grid, dim3(32 * kRowsWarps), 0, s, 0, a);
+  const int nout = a.act == 2 ? a.N / 2 : a.N, kp = mx_kp(a.K);
+  const dim3 grid((nout + kRowsWarps - 1) / kRowsWarps);
+  const size_t smem = (size_t)MB * (kp / 2 + kp / 8);
+  auto k = a.x ? (a.act == 2 ? mx4_rows_kernel<T, MB, true, true> : mx4_rows_kernel<T, MB, false, true>)
+               : (a.act == 2 ? mx4_rows_kernel<T, MB, true, false> : mx4_rows_kernel<T, MB, false, false>);
+  return launch_kernel(k, grid, dim3(kRowsThreads), smem, s, 0, a);
 }
 
 // ------------------------------------------------------------------ tensor-core product
@@ -111,15 +201,14 @@ cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
 //               scale tiles by untiled bulk copies (a tile's 512 bytes are contiguous)
 //   warp 1      TMEM allocator and issuer: per stage the scale tiles into TMEM (tcgen05.cp), then up to four
 //               tcgen05.mma.kind::mxf4 (K = 64); copies and MMAs of one thread execute in order
-//   warps 2..9  epilogue, two per TMEM lane quadrant: 32 rows x 64 accumulator columns at a time through a
-//               swizzled shared-memory panel that TMA fills with the residual beforehand and stores from afterwards,
-//               so global memory is only touched in full lines and never waited for by the arithmetic
-// Accumulators are double-buffered in TMEM. n is the fastest tile index: the tiles in flight share rows of x, and w
+//   others      epilogue, two sets of BN / 16 warps that take turns on the tiles (the activations would otherwise be
+//               bound by too few warps to hide their latencies: GEGLU 8192 x 2560 x 320 ran 18.5 us with one set). A warp
+//               takes 32 rows x 64 accumulator columns through a swizzled shared-memory panel that TMA fills with the
+//               residual beforehand and stores from afterwards, so global memory is only touched in full lines
+// Accumulators are double-buffered in TMEM, one per set. n is the fastest tile index: the tiles in flight share rows of x, and w
 // (at most a few MB) stays in L2.
 constexpr int kGBM = 128;
 constexpr int kGStageCols = 256;  // K columns per stage: one 128-byte swizzled row of codes
-constexpr int kGEpiWarps = 8;
-constexpr int kGThreads = 64 + 32 * kGEpiWarps;
 
 template <int BN, bool GEGLU>
 struct GCfg {
@@ -129,13 +218,15 @@ struct GCfg {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr int kPW = GEGLU ? 32 : 64;                 // output columns of a panel (64 accumulator columns)
   static constexpr uint32_t kPanelBytes = 32 * kPW * 2;
-  static constexpr int kHalves = BN >= 128 ? 2 : 1;           // BN = 64: the two warps of a quadrant take turns on tiles
-  static constexpr uint32_t kTail = kGEpiWarps * 64 * 4 + 512;  // bias, barriers, TMEM slot
-  static constexpr int kStages = (232448 - 1024 - kTail - 2 * kGEpiWarps * kPanelBytes) / kStageBytes;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + 2 * kGEpiWarps * kPanelBytes + kTail;
+  static constexpr int kSetWarps = 4 * (BN / 64), kEpiWarps = 2 * kSetWarps;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr uint32_t kTail = kEpiWarps * 64 * 4 + 512;  // bias, barriers, TMEM slot
+  static constexpr int kStages = (232448 - 1024 - kTail - kEpiWarps * kPanelBytes) / kStageBytes;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kEpiWarps * kPanelBytes + kTail;
   static constexpr uint32_t kSfCols = 8 + 8 * kBTiles;        // TMEM columns of one stage's scales
   static constexpr uint32_t kTmemCols = 2 * BN + 2 * kSfCols <= 256 ? 256 : 512;
   static_assert(2 * BN + 2 * kSfCols <= 512 && kStages >= 3, "tile does not fit");
+  static_assert((2 * kStages + 5 + kEpiWarps) * 8 + 4 <= 512, "barriers do not fit");
 };
 
 struct GemmMx4Dev {
@@ -148,7 +239,7 @@ struct GemmMx4Dev {
 };
 
 template <int BN, typename T, int ACT>
-__global__ void __launch_bounds__(kGThreads, 1)
+__global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
                     const GemmMx4Dev p) {
@@ -158,10 +249,10 @@ __global__ void __launch_bounds__(kGThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sPanel = smem + S * (C::kABytes + C::kBBytes);
-  uint8_t* sSf = sPanel + 2 * kGEpiWarps * C::kPanelBytes;
+  uint8_t* sSf = sPanel + C::kEpiWarps * C::kPanelBytes;
   float* sBias = reinterpret_cast<float*>(sSf + S * C::kSfBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sBias + kGEpiWarps * 64);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + 2 * kGEpiWarps);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sBias + C::kEpiWarps * 64);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + C::kEpiWarps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -169,7 +260,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
   auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * S + a); };
   auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
   const uint32_t drain_bar = bar0 + 8u * (2 * S + 4);
-  auto res_bar = [&](int w, int b) { return bar0 + 8u * (2 * S + 5 + 2 * w + b); };
+  auto res_bar = [&](int w) { return bar0 + 8u * (2 * S + 5 + w); };
 
   const int num_m = (p.M + kGBM - 1) / kGBM, num_n = (p.N + BN - 1) / BN;
   const long long num_tiles = (long long)num_m * num_n;
@@ -183,11 +274,10 @@ __global__ void __launch_bounds__(kGThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), C::kHalves * 4);
+      mbar_init(tempty_bar(a), C::kSetWarps);
     }
     mbar_init(drain_bar, 1);
-    for (int w = 0; w < kGEpiWarps; ++w)
-      for (int b = 0; b < 2; ++b) mbar_init(res_bar(w, b), 1);
+    for (int w = 0; w < C::kEpiWarps; ++w) mbar_init(res_bar(w), 1);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -278,119 +368,106 @@ __global__ void __launch_bounds__(kGThreads, 1)
     }
   } else {
     pdl_wait();
-    const int w = warp - 2, lg = warp & 3, half = w >> 2;
-    const int rl = lg * 32 + lane;
+    // set: which tiles (and accumulator); lg: the TMEM lane quadrant a warp may read; pn: its 64 columns
+    const int w = warp - 2, set = w / C::kSetWarps, lg = warp & 3, pn = (w % C::kSetWarps) >> 2;
     float* bias_s = sBias + w * 64;
-    constexpr int kPanels = BN / 64;                // panels of a tile
-    constexpr int kStep = C::kHalves;               // this warp's panels: half, half + kStep, ...
-    const int first = kStep == 2 ? half : 0;
-    uint8_t* pan0 = sPanel + (w * 2) * C::kPanelBytes;
-    // the panel after (tile, pn): the next of this tile, else the first of this warp's next tile
-    const long long tstep = kStep == 2 ? gridDim.x : 2ll * gridDim.x;
-    const long long tfirst = kStep == 2 ? blockIdx.x : blockIdx.x + (long long)half * gridDim.x;
-    uint32_t q = 0, tl = kStep == 2 ? 0 : (uint32_t)half;
-    auto load_res = [&](long long tile, int pn, uint32_t b) {  // lane 0
-      mbar_arrive_expect_tx(res_bar(w, b), C::kPanelBytes);
-      tma_load_2d(smem_u32(pan0 + b * C::kPanelBytes), &map_r, res_bar(w, b), (int)(tile % num_n) * BN + pn * 64,
+    uint8_t* pan = sPanel + w * C::kPanelBytes;
+    const long long tstep = 2ll * gridDim.x;
+    auto load_res = [&](long long tile) {  // lane 0
+      mbar_arrive_expect_tx(res_bar(w), C::kPanelBytes);
+      tma_load_2d(smem_u32(pan), &map_r, res_bar(w), (int)(tile % num_n) * BN + pn * 64,
                   (int)(tile / num_n) * kGBM + lg * 32);
     };
-    if (p.residual && lane == 0 && tfirst < num_tiles) load_res(tfirst, first, 0);
-    bool ok = true;
-    for (long long tile = tfirst; tile < num_tiles; tile += tstep, tl += 3 - kStep) {
-      const uint32_t acc = tl & 1u;
-      const int m0 = (int)(tile / num_n) * kGBM, n0 = (int)(tile % num_n) * BN;
-      ok = mbar_wait(tfull_bar(acc), (tl >> 1) & 1u, p.err, kDevTimeoutAcc);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+    long long tile = blockIdx.x + (long long)set * gridDim.x;
+    bool loading = false;  // a residual copy of this warp is in flight (lane 0)
+    if (p.residual && lane == 0 && tile < num_tiles) {
+      load_res(tile);
+      loading = true;
+    }
+    for (uint32_t q = 0; tile < num_tiles; tile += tstep, ++q) {
+      const int m0 = (int)(tile / num_n) * kGBM, n = (int)(tile % num_n) * BN + pn * 64;
+      bias_s[lane] = p.bias && n + lane < p.N ? p.bias[n + lane] : 0.f;
+      bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? p.bias[n + 32 + lane] : 0.f;
+      if (!p.residual && lane == 0) bulk_wait_read<0>();  // the panel's previous store has read it
+      __syncwarp();
+      bool ok = mbar_wait(tfull_bar(set), q & 1u, p.err, kDevTimeoutAcc);
+      if (ok && p.residual) {
+        ok = mbar_wait(res_bar(w), q & 1u, p.err, kDevTimeoutEmpty);
+        if (ok) loading = false;
+      }
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-#pragma unroll 1
-      for (int pn = first; pn < kPanels; pn += kStep, ++q) {
-        const uint32_t b = q & 1u;
-        uint8_t* pan = pan0 + b * C::kPanelBytes;
-        const int n = n0 + pn * 64;
-        if (lane == 0) {
-          if (p.residual) {
-            bulk_wait_read<0>();  // the other buffer's store has read it: it may take the next residual
-            const bool more = pn + kStep < kPanels;
-            const long long nt = more ? tile : tile + tstep;
-            if (nt < num_tiles) load_res(nt, more ? pn + kStep : first, b ^ 1u);
-          } else {
-            bulk_wait_read<1>();  // this buffer's previous store has read it
-          }
-        }
-        bias_s[lane] = p.bias && n + lane < p.N ? p.bias[n + lane] : 0.f;
-        bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? p.bias[n + 32 + lane] : 0.f;
-        __syncwarp();
-        if (p.residual) {
-          ok = mbar_wait(res_bar(w, b), (q >> 1) & 1u, p.err, kDevTimeoutEmpty);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        }
-        const uint32_t t_row = tmem_base + acc * BN + pn * 64 + (static_cast<uint32_t>(lg * 32) << 16);
+      const uint32_t t_row = tmem_base + set * BN + pn * 64 + (static_cast<uint32_t>(lg * 32) << 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
-          tmem_ld32(t_row + 32 * h, r);
-          tmem_wait_ld();
-          const float4* b4 = reinterpret_cast<const float4*>(bias_s + 32 * h);
-          if constexpr (GEGLU) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              float v[8];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float4 bv = b4[2 * g + e], bg = b4[4 + 2 * g + e];
-                const int i = 8 * g + 4 * e;
-                v[4 * e] = (__uint_as_float(r[i]) + bv.x) * gelu_as(__uint_as_float(r[16 + i]) + bg.x);
-                v[4 * e + 1] = (__uint_as_float(r[i + 1]) + bv.y) * gelu_as(__uint_as_float(r[17 + i]) + bg.y);
-                v[4 * e + 2] = (__uint_as_float(r[i + 2]) + bv.z) * gelu_as(__uint_as_float(r[18 + i]) + bg.z);
-                v[4 * e + 3] = (__uint_as_float(r[i + 3]) + bv.w) * gelu_as(__uint_as_float(r[19 + i]) + bg.w);
-              }
-              // 64-byte rows: 16-byte chunk index XOR address bits 7..8
-              mx_store8<T>(reinterpret_cast<T*>(pan + lane * 64 + (((2 * h + g) ^ ((lane >> 1) & 3)) << 4)), v);
-            }
-          } else {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              // 128-byte rows: 16-byte chunk index XOR address bits 7..9
-              T* at = reinterpret_cast<T*>(pan + lane * 128 + (((4 * h + g) ^ (lane & 7)) << 4));
-              const float4 b0 = b4[2 * g], b1 = b4[2 * g + 1];
-              float v[8] = {__uint_as_float(r[8 * g]) + b0.x,     __uint_as_float(r[8 * g + 1]) + b0.y,
-                            __uint_as_float(r[8 * g + 2]) + b0.z, __uint_as_float(r[8 * g + 3]) + b0.w,
-                            __uint_as_float(r[8 * g + 4]) + b1.x, __uint_as_float(r[8 * g + 5]) + b1.y,
-                            __uint_as_float(r[8 * g + 6]) + b1.z, __uint_as_float(r[8 * g + 7]) + b1.w};
-              if (p.residual) {
-                float rv[8];
-                mx_unpack8<T>(*reinterpret_cast<const uint4*>(at), rv);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += rv[i];
-              }
-              if constexpr (ACT == 1) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = silu_fine(v[i]);
-              }
-              mx_store8<T>(at, v);
-            }
-          }
-        }
-        if (pn + kStep >= kPanels) {  // the accumulator's last read of this warp
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        tmem_ld32(t_row + 32 * h, r);
+        tmem_wait_ld();
+        if (h == 1) {  // the accumulator's last read of this warp
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty_bar(acc));
+          if (lane == 0) mbar_arrive(tempty_bar(set));
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&map_y, smem_u32(pan), GEGLU ? n / 2 : n, m0 + lg * 32);
-          bulk_commit();
+        const float4* b4 = reinterpret_cast<const float4*>(bias_s + 32 * h);
+        auto acc2 = [&](int i, float x, float y) {
+          return add_f32x2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(x, y));
+        };
+        if constexpr (GEGLU) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float4 bv = b4[2 * g + e], bg = b4[4 + 2 * g + e];
+              const int i = 8 * g + 4 * e;
+              const float2 lo = mul_f32x2(acc2(i, bv.x, bv.y), gelu_pair(acc2(16 + i, bg.x, bg.y)));
+              const float2 hi = mul_f32x2(acc2(i + 2, bv.z, bv.w), gelu_pair(acc2(18 + i, bg.z, bg.w)));
+              v[4 * e] = lo.x; v[4 * e + 1] = lo.y; v[4 * e + 2] = hi.x; v[4 * e + 3] = hi.y;
+            }
+            // 64-byte rows: 16-byte chunk index XOR address bits 7..8
+            mx_store8<T>(reinterpret_cast<T*>(pan + lane * 64 + (((2 * h + g) ^ ((lane >> 1) & 3)) << 4)), v);
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            // 128-byte rows: 16-byte chunk index XOR address bits 7..9
+            T* at = reinterpret_cast<T*>(pan + lane * 128 + (((4 * h + g) ^ (lane & 7)) << 4));
+            const float4 b0 = b4[2 * g], b1 = b4[2 * g + 1];
+            float2 u[4] = {acc2(8 * g, b0.x, b0.y), acc2(8 * g + 2, b0.z, b0.w), acc2(8 * g + 4, b1.x, b1.y),
+                           acc2(8 * g + 6, b1.z, b1.w)};
+            if (p.residual) {
+              float rv[8];
+              mx_unpack8<T>(*reinterpret_cast<const uint4*>(at), rv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) u[i] = add_f32x2(u[i], make_float2(rv[2 * i], rv[2 * i + 1]));
+            }
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[2 * i] = ACT == 1 ? silu_fine(u[i].x) : u[i].x;
+              v[2 * i + 1] = ACT == 1 ? silu_fine(u[i].y) : u[i].y;
+            }
+            mx_store8<T>(at, v);
+          }
         }
       }
-      if (!ok) break;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(&map_y, smem_u32(pan), GEGLU ? n / 2 : n, m0 + lg * 32);
+        bulk_commit();
+        if (p.residual && tile + tstep < num_tiles) {  // the panel takes the next residual once the store has read it
+          bulk_wait_read<0>();
+          load_res(tile + tstep);
+          loading = true;
+        }
+      }
     }
     if (lane == 0) {
-      // abort: the residual loads in flight (panel q's, and q + 1's where it was issued) land first
-      if (!ok && p.residual) spin_ns(200000);
+      // abort: a residual copy in flight lands before the shared memory is released
+      if (loading) spin_ns(200000);
       bulk_wait_read<0>();
     }
-    (void)rl;
   }
   tc_fence_before();
   __syncthreads();
@@ -435,7 +512,7 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   p.xs = a.xscales; p.ws = a.wscales; p.bias = a.bias; p.residual = a.residual != nullptr; p.err = err;
   const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + BN - 1) / BN);
   const int grid = (int)std::min<long long>(tiles, num_sms());
-  return launch_kernel(k, dim3(grid), dim3(kGThreads), C::kSmem, s, 0, mx, mw, my, mr, p);
+  return launch_kernel(k, dim3(grid), dim3(C::kThreads), C::kSmem, s, 0, mx, mw, my, mr, p);
 }
 
 template <typename T, int ACT>
@@ -447,8 +524,9 @@ cudaError_t gemm_bn(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 
 template <typename T>
 cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  if (a.M == 1) return launch_rows<T, 1>(a, s);
-  if (a.M <= 8) return launch_rows<T, 4>(a, s);
+  if (mx4_linear_rows(a.M, a.K)) {
+    return a.M == 1 ? launch_rows<T, 1>(a, s) : a.M == 2 ? launch_rows<T, 2>(a, s) : a.M <= 4 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
+  }
   switch (a.act) {
     case 1: return gemm_bn<T, 1>(a, err, s);
     case 2: return gemm_bn<T, 2>(a, err, s);
@@ -457,6 +535,9 @@ cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Few rows run on the CUDA cores, as long as their operand fits 48 KB of shared memory.
+bool mx4_linear_rows(int M, int K) { return M <= 8 && (size_t)8 * (mx_kp(K) / 2 + mx_kp(K) / 8) <= 48 * 1024; }
 
 cudaError_t launch_mx4_linear(const Mx4LinearArgs& a, int* dev_err, cudaStream_t s) {
   return a.dtype == kBF16 ? linear_t<__nv_bfloat16>(a, dev_err, s) : linear_t<__half>(a, dev_err, s);
