@@ -293,7 +293,9 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  pdl_trigger();
+  // No early trigger: blocks of the next kernel that move in while this one runs hold their SMs' warps and registers
+  // unevenly when it ends. Measured on B200, quantise + product in a row: 65536 x 640 x 2560 181 us with a trigger here,
+  // 163 us with one after the last MMA, 161 us without; 8192 x 320 x 320 9.3 / 8.3 / 7.8 us.
 
   if (warp == 0) {
     if (lane == 0) {

@@ -219,12 +219,13 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
 // Two launches. Statistics: each block reads one chunk of an image's pixels (about 32 KB, all channels) once and
 // writes each group's (mean, M2 = sum of squared differences from that mean) over the chunk. Apply: each block
 // merges the chunks' pairs of the groups its tiles need, in chunk order, then normalises, activates and quantises one to
-// four tiles of the same channels (as many as leave four blocks per SM). Threads' and chunks' pairs merge by Chan,
+// four tiles of the same channels. Threads' and chunks' pairs merge by Chan,
 // Golub and LeVeque's update of (n, mean, M2). Chunks depend on (HW, C) alone: an image's result does
 // not depend on the batch, and no atomics make the order of a sum vary. The second read of x comes from L2 while an
 // input fits it.
 constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 8;         // pixels a thread holds at once
+constexpr int kGnShift = 4;         // pixels that give the shift
 constexpr int kGnPixels = 16;       // pixels per thread and chunk, more where an image would need over kGnMaxChunks
 constexpr int kGnMaxC = 4096;
 constexpr int kGnMaxChunks = 256;
@@ -233,6 +234,11 @@ constexpr int kGnMaxChunks = 256;
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -250,9 +256,9 @@ GnPlan gn_plan(int HW, int C) {
   return p;
 }
 
-// A thread sums d and d^2 of its n pixels of a channel, d = x - k with k the mean of its first m = min(n, 8) pixels.
+// A thread sums d and d^2 of its n pixels of a channel, d = x - k with k the mean of its first m = min(n, 4) pixels.
 // (k - mean)^2 <= M2 / m (Cauchy), so sum d^2 <= M2 (1 + n / m) and M2 = sum d^2 - (sum d)^2 / n loses at most the
-// factor 1 + n / m (3 at 16 pixels) to cancellation, whatever the data.
+// factor 1 + n / m (5 at 16 pixels) to cancellation, whatever the data.
 template <typename T>
 __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
                                                                   int chunk, float2* part) {
@@ -283,12 +289,12 @@ __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x,
       }
       if (i0 == 0) {
 #pragma unroll
-        for (int i = 0; i < kGnBatch; ++i) {
+        for (int i = 0; i < kGnShift; ++i) {
           const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) k[e] = add_f32x2(k[e], MxElem<T>::get2(w[e]));
         }
-        const float inv = 1.f / (float)nb;
+        const float inv = 1.f / (float)min(kGnShift, nb);
 #pragma unroll
         for (int e = 0; e < 4; ++e) k[e] = mul_f32x2(k[e], make_float2(inv, inv));
       }
@@ -315,40 +321,33 @@ __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x,
     }
   }
   __syncthreads();
-  const int rows = p1 - p0;
-  if (par > 1) {  // per channel, the thread rows' pairs (row rr holds every par-th pixel) into row 0
-    for (int c = threadIdx.x; c < C; c += kGnThreads) {
-      float2 a = acc[c];
-      float n = (float)((rows + par - 1) / par);
-      for (int rr = 1; rr < par && rr < rows; ++rr) {
-        const float2 b = acc[rr * C + c];
-        const float nb = (float)((rows - rr + par - 1) / par), w = nb / (n + nb), d = b.x - a.x;
-        a.x = fmaf(d, w, a.x);
-        a.y += b.y + d * d * w * n;
-        n += nb;
-      }
-      acc[c] = a;
-    }
-    __syncthreads();
-  }
-  // one warp per group: its cpg channels, `rows` pixels each
-  const int lane = threadIdx.x & 31;
-  const float inv_cpg = 1.f / (float)cpg;
-  for (int g = threadIdx.x >> 5; g < groups; g += kGnThreads / 32) {
+  // eight lanes per group: its par x cpg pairs, thread row rr holding q or q + 1 pixels
+  const int rows = p1 - p0, q = rows / par, rem = rows - q * par, sub = threadIdx.x & 7;
+  const float inv_n = 1.f / ((float)rows * cpg);
+  for (int g = threadIdx.x >> 3; g < (groups + 3) / 4 * 4; g += kGnThreads / 8) {  // whole warps: the shuffles need them
+    const float2* a = acc + min(g, groups - 1) * cpg;
     float s = 0.f;
-    for (int i = lane; i < cpg; i += 32) s += acc[g * cpg + i].x;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mu = s * inv_cpg;
-    float m2 = 0.f;
-    for (int i = lane; i < cpg; i += 32) {
-      const float2 a = acc[g * cpg + i];
-      const float d = a.x - mu;
-      m2 += fmaf((float)rows * d, d, a.y);
+    for (int rr = 0; rr < par; ++rr) {
+      const float n = (float)(q + (rr < rem));
+      if (n != 0.f)
+        for (int i = sub; i < cpg; i += 8) s = fmaf(n, a[rr * C + i].x, s);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
-    if (lane == 0) part[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * groups + g] = make_float2(mu, m2);
+    for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float mu = s * inv_n;
+    float m2 = 0.f;
+    for (int rr = 0; rr < par; ++rr) {
+      const float n = (float)(q + (rr < rem));
+      if (n != 0.f)
+        for (int i = sub; i < cpg; i += 8) {
+          const float2 v = a[rr * C + i];
+          const float d = v.x - mu;
+          m2 += fmaf(n * d, d, v.y);
+        }
+    }
+#pragma unroll
+    for (int o = 4; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+    if (sub == 0 && g < groups) part[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * groups + g] = make_float2(mu, m2);
   }
 }
 
@@ -379,7 +378,8 @@ __device__ __forceinline__ float2 gn_merge(const float2* part, int g, int groups
 // nothing next to a block maximum that is not itself below 2^-40.
 __device__ __forceinline__ float2 silu_pair(float2 y) {
   const float2 t = mul_f32x2(y, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  const float a = fminf(1.f + ex2_approx(t.x), 9.2233720e18f), b = fminf(1.f + ex2_approx(t.y), 9.2233720e18f);
+  const float2 s = add_f32x2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
+  const float a = fminf(s.x, 9.2233720e18f), b = fminf(s.y, 9.2233720e18f);
   const float r = rcp_approx(a * b);
   return mul_f32x2(y, mul_f32x2(make_float2(r, r), make_float2(b, a)));
 }
@@ -467,34 +467,49 @@ __global__ void __launch_bounds__(kQThreads, 3) mx4_gn_apply_kernel(const T* x, 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < Q::kPass; ++i) {
-      const int rl = i * Q::kRows + r0, r = row0 + rl;
-      const int img = imgs == 1 ? img0 : min(r, p.M - 1) / p.HW;
-      const float4* fac = reinterpret_cast<const float4*>(affine + (img - img0) * 2 * kMxTileCols + l * 4);
-      float v[16];
-      float top = 0.f;
+    for (int i = 0; i < Q::kPass; i += 2) {  // two rows at a time: they share the factors' loads where they share an image
+      float v[2][16], top[2] = {0.f, 0.f};
+      int rl[2], img[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        rl[h] = (i + h) * Q::kRows + r0;
+        img[h] = imgs == 1 ? img0 : min(row0 + rl[h], p.M - 1) / p.HW;
+      }
+      const float4* fac0 = reinterpret_cast<const float4*>(affine + (img[0] - img0) * 2 * kMxTileCols + l * 4);
+      const float4* fac1 = reinterpret_cast<const float4*>(affine + (img[1] - img0) * 2 * kMxTileCols + l * 4);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float4 f;
+        float4 f[2];
         if constexpr (FEW) {
-          const int c0 = min(c + 2 * j, p.C - 2);
-          const float2 f0 = factors(c0, one_chunk(img, c0 / cpg)), f1 = factors(c0 + 1, one_chunk(img, (c0 + 1) / cpg));
-          f = c + 2 * j < p.C ? make_float4(f0.x, f1.x, f0.y, f1.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c0 = min(c + 2 * j, p.C - 2);
+            const float2 a = factors(c0, one_chunk(img[h], c0 / cpg)), b = factors(c0 + 1, one_chunk(img[h], (c0 + 1) / cpg));
+            f[h] = c + 2 * j < p.C ? make_float4(a.x, b.x, a.y, b.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
         } else {
-          f = fac[8 * j];
+          f[0] = fac0[8 * j];
+          f[1] = imgs == 1 ? f[0] : fac1[8 * j];
         }
-        float2 y = fma_f32x2(MxElem<T>::get2(raw[i].w[j]), make_float2(f.x, f.y), make_float2(f.z, f.w));
-        if constexpr (SILU) y = silu_pair(y);
-        v[2 * j] = y.x;
-        v[2 * j + 1] = y.y;
-        top = max_nan(top, max_nan(fabsf(y.x), fabsf(y.y)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float2 y = fma_f32x2(MxElem<T>::get2(raw[i + h].w[j]), make_float2(f[h].x, f[h].y), make_float2(f[h].z, f[h].w));
+          if constexpr (SILU) y = silu_pair(y);
+          v[h][2 * j] = y.x;
+          v[h][2 * j + 1] = y.y;
+          top[h] = max_nan(top[h], fabsf(y.x), fabsf(y.y));
+        }
       }
-      uint32_t m = __float_as_uint(top) & 0x7FFFFFFFu;
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      const uint32_t e = mx_exponent(m);
-      uint32_t q[2];
-      mx_codes<16>(v, e, q);
-      if (r < p.M && c < kp) put_codes<T>(q, e, l, rl, c, p.codes + (size_t)r * (kp / 2), tile);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + rl[h];
+        uint32_t m = __float_as_uint(top[h]) & 0x7FFFFFFFu;
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const uint32_t e = mx_exponent(m);
+        uint32_t q[2];
+        mx_codes<16>(v[h], e, q);
+        if (r < p.M && c < kp) put_codes<T>(q, e, l, rl[h], c, p.codes + (size_t)r * (kp / 2), tile);
+      }
     }
     __syncthreads();
     if (threadIdx.x < kMxTileBytes / 4)
@@ -560,7 +575,13 @@ cudaError_t groupnorm_t(const Mx4GroupNormArgs& a, cudaStream_t s) {
   };
   auto k = a.HW <= kGnPixels ? pick(std::true_type()) : pick(std::false_type());
   const int rts = mx_rtiles(p.M), kts = mx_ktiles(a.C);
-  p.tiles = (int)std::max<long long>(1, std::min<long long>(4, (long long)rts * kts / (4 * num_sms())));
+  // tiles per block: fewest rounds of blocks (three per SM) weighted by a block's work, a merge counting half a tile
+  double best = 1e30;
+  for (int n = 1; n <= 4; ++n) {
+    const long long blocks = (long long)((rts + n - 1) / n) * kts, slots = 3ll * num_sms();
+    const double cost = (double)((blocks + slots - 1) / slots) * (n + 0.5);
+    if (cost < best) { best = cost; p.tiles = n; }
+  }
   return launch_kernel(k, dim3((rts + p.tiles - 1) / p.tiles * kts), dim3(kQThreads), 0, s, 0, x, p);
 }
 
