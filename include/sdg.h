@@ -326,13 +326,14 @@ SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M,
                            const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,
                            void* y, int* err_word, void* stream);
 
-/* The same with x [M, K] of type dtype (row stride ldx elements), quantised on the way into scratch
- * (sdg_linear_mx4_scratch_bytes(M, K) bytes, 16-byte aligned; its contents on entry do not matter; a few rows
- * need none: 0 bytes, scratch may be NULL). */
+/* The same with x [M, K] of type dtype (row stride ldx elements), quantised on the way: in the
+ * same launch for few rows and for small products of 16-byte aligned rows (sdg_linear_mx4_scratch_bytes of the same
+ * arguments returns 0 and scratch may be NULL), else into scratch of that many bytes, 16-byte aligned, whose contents
+ * on entry do not matter. */
 SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales,
                              const float* bias, int N, const void* residual, int act, int dtype, void* y, void* scratch,
                              size_t scratch_bytes, int* err_word, void* stream);
-SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K);
+SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N);
 
 /* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
  * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to

@@ -103,7 +103,7 @@ _SIGS = {
     "sdg_dequantize_mx4": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "sdg_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P]),
     "sdg_linear_mx4_x": (_I, [_P, _I, _I, ctypes.c_int64, _P, _P, _P, _I, _P, _I, _I, _P, _P, ctypes.c_size_t, _P, _P]),
-    "sdg_linear_mx4_scratch_bytes": (ctypes.c_size_t, [_I, _I]),
+    "sdg_linear_mx4_scratch_bytes": (ctypes.c_size_t, [_P, _I, _I, ctypes.c_int64, _I]),
     "sdg_groupnorm_mx4": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
     "sdg_groupnorm_mx4_scratch_bytes": (ctypes.c_size_t, [_I, _I, _I, _I]),
     "sdg_upsample_conv3x3": (_I, [_P, _I, _I, _I, _I, _P, _P, _I, _P, _P, ctypes.c_size_t, _P, _P]),
@@ -536,13 +536,14 @@ def _mx4_rows(x):
     return R, K, ldx if R > 1 else K
 
 
-def _mx4_operand(out, rows: int, half: int, like, dev: int):
-    """The (codes, scales) pair to write into, with both pointers."""
+def _mx4_operand(out, rows: int, half: int, like, dev: int, extra: int = 0):
+    """The (codes, scales) pair to write into, with both pointers; a pair allocated here has ``extra`` bytes behind it."""
     U8 = _torch.uint8
-    if out is None:
-        codes = like.new_empty((rows, half), dtype=U8)
-        scales = like.new_empty(_mx4_scale_shape(rows, half), dtype=U8)
-        return codes, scales, codes.data_ptr(), scales.data_ptr()
+    if out is None:  # one allocation for both arrays (the scales on a 512-byte boundary behind the codes)
+        rt, kt, n = (rows + 127) // 128, (half + 63) // 64, (rows * half + 511) // 512 * 512
+        both = like.new_empty(n + rt * kt * 512 + extra, dtype=U8)
+        p = both.data_ptr()
+        return both.as_strided((rows, half), (half, 1)), both.as_strided((rt, kt, 512), (kt * 512, 512, 1), n), p, p + n
     codes, scales = out
     return (codes, scales, _mx4_arg(codes, "codes", dev, U8, (rows, half)),
             _mx4_arg(scales, "scales", dev, U8, _mx4_scale_shape(rows, half)))
@@ -623,12 +624,12 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
     else:
         py = _mx4_arg(out, "out", dev, dt, shape)
     if xscale is None:
-        ps, nb = None, lib().sdg_linear_mx4_scratch_bytes(M, K)
+        px, ps, L = x.data_ptr(), None, lib()
+        nb = L.sdg_linear_mx4_scratch_bytes(px, M, K, ldx, N)
         if nb:
-            scratch = x.new_empty((nb,), dtype=U8)
+            scratch = x.new_empty(nb, dtype=U8)
             ps = scratch.data_ptr()
-        _mx4_call(lib().sdg_linear_mx4_x, dev, x.data_ptr(), M, K, ldx, pw, pws, pb, N, pr, act, code, py,
-                  ps, nb, pe)
+        _mx4_call(L.sdg_linear_mx4_x, dev, px, M, K, ldx, pw, pws, pb, N, pr, act, code, py, ps, nb, pe)
     else:
         px = _mx4_arg(x, "x codes", dev, U8, (M, half))
         pxs = _mx4_arg(xscale, "xscale", dev, U8, _mx4_scale_shape(M, half))
@@ -650,13 +651,17 @@ def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=
     px = _mx4_arg(x, "x", dev, x.dtype, (B, HW, C))
     pg = _mx4_arg(gamma, "gamma", dev, T.float32, (C,))
     pb = _mx4_arg(beta, "beta", dev, T.float32, (C,))
-    codes, scales, pc, ps = _mx4_operand(out, B * HW, (C + 31) // 32 * 16, x, dev)
-    need = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups)
-    if stats is None:
-        stats = x.new_empty((need // 4 + 1,), dtype=T.float32)
-    pt = _mx4_arg(stats, "stats", dev, T.float32, stats.shape)
-    if stats.numel() * 4 < need:
-        raise SdgError(2, f"stats: {need} bytes are needed")
+    need, half = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups), (C + 31) // 32 * 16
+    codes, scales, pc, ps = _mx4_operand(out, B * HW, half, x, dev, need if stats is None else 0)
+    if stats is not None:
+        pt = _mx4_arg(stats, "stats", dev, T.float32, stats.shape)
+        if stats.numel() * 4 < need:
+            raise SdgError(2, f"stats: {need} bytes are needed")
+    elif out is None:
+        pt = ps + scales.numel()
+    else:
+        stats = x.new_empty(need // 4 + 1, dtype=T.float32)
+        pt = stats.data_ptr()
     _mx4_call(lib().sdg_groupnorm_mx4, dev, px, dt, B, HW, C, groups, pg, pb, eps,
               int(silu), pc, ps, pt)
     return codes, scales

@@ -126,13 +126,12 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
                              size_t scratch_bytes, int* err_word, void* stream) {
   int st = linear_check("linear_mx4", M, K, wcodes, wscales, bias, N, residual, act, dtype, y);
   if (st) return st;
-  const bool rows = sdg::mx4_linear_rows(M, K);
-  const size_t need = sdg_linear_mx4_scratch_bytes(M, K);
+  const size_t need = sdg_linear_mx4_scratch_bytes(x, M, K, ldx, N);
   if (!x || ldx < 0 || !aligned(x, 2) || (need && (!scratch || !aligned(scratch, 16) || scratch_bytes < need)))
     return op_fail(SDG_ERR_ARG, "linear_mx4: bad x, or scratch smaller than sdg_linear_mx4_scratch_bytes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   sdg::Mx4LinearArgs a;
-  if (rows) {
+  if (need == 0) {
     a.x = x;
     a.ldx = ldx;
   } else {
@@ -146,8 +145,8 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
   return linear_run(a, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word, s);
 }
 
-SDG_API size_t sdg_linear_mx4_scratch_bytes(int M, int K) {
-  if (M <= 0 || K <= 0 || K > kMaxK || sdg::mx4_linear_rows(M, K)) return 0;
+SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK || sdg::mx4_linear_takes_x(x, M, K, ldx, N)) return 0;
   return code_space(M, K) + sdg_mx4_scale_bytes(M, K);
 }
 

@@ -197,6 +197,9 @@ cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
 
 // ------------------------------------------------------------------ tensor-core product
 // mx4_gemm_kernel: persistent, warp-specialised, one CTA per SM, 128 x BN output tiles.
+// The producer's and the issuer's loops run on all lanes with one elected lane issuing: the operands then stay in uniform
+// registers. With the loops on one lane (a divergent branch) every tcgen05 instruction paid for moving its operands
+// there: 65536 x 640 x 2560 94 us, 76 us with the issuer converted, 72.6 us with both.
 //   warp 0      producer: per stage (256 columns of K) the 128 B-swizzled code tiles of x and w by TMA, and their
 //               scale tiles by untiled bulk copies (a tile's 512 bytes are contiguous)
 //   warp 1      TMEM allocator and issuer: per stage the scale tiles into TMEM (tcgen05.cp), then up to four
@@ -205,12 +208,21 @@ cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
 //               bound by too few warps to hide their latencies: GEGLU 8192 x 2560 x 320 ran 18.5 us with one set). A warp
 //               takes 32 rows x 64 accumulator columns through a swizzled shared-memory panel that TMA fills with the
 //               residual beforehand and stores from afterwards, so global memory is only touched in full lines
-// Accumulators are double-buffered in TMEM, one per set. n is the fastest tile index: the tiles in flight share rows of x, and w
+// Accumulators are double-buffered in TMEM, one per set.
+// FUSE (BN = 64): x is quantised on the way, so the call is one launch without scratch: one more warp brings tiles of
+// 128 rows x 128 columns of x into a ring by TMA and sixteen more quantise them into the code stages. (Loading x into
+// registers a stage ahead instead ran four times slower: the loads in flight share the scoreboard that the pass in
+// hand waits on.) Every n tile quantises its rows of x again: for small products only.
+// n is the fastest tile index: the tiles in flight share rows of x, and w
 // (at most a few MB) stays in L2.
 constexpr int kGBM = 128;
 constexpr int kGStageCols = 256;  // K columns per stage: one 128-byte swizzled row of codes
 
-template <int BN, bool GEGLU>
+constexpr int kGQuantWarps = 16;
+constexpr int kGRawStages = 3;
+constexpr uint32_t kGRawBytes = kGBM * 128 * 2;  // 128 columns of 16 bits, as two 128 B-swizzled boxes of 64
+
+template <int BN, bool GEGLU, bool FUSE>
 struct GCfg {
   static constexpr int kBTiles = (BN + kMxTileRows - 1) / kMxTileRows;  // scale tiles of w per 128 columns of K
   static constexpr uint32_t kABytes = kGBM * 128, kBBytes = BN * 128;
@@ -218,15 +230,19 @@ struct GCfg {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr int kPW = GEGLU ? 32 : 64;                 // output columns of a panel (64 accumulator columns)
   static constexpr uint32_t kPanelBytes = 32 * kPW * 2;
-  static constexpr int kSetWarps = 4 * (BN / 64), kEpiWarps = 2 * kSetWarps;
-  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static_assert(!FUSE || BN == 64, "the fused form has 64-wide tiles");
+  static constexpr int kSets = FUSE ? 1 : 2;
+  static constexpr int kSetWarps = 4 * (BN / 64), kEpiWarps = kSets * kSetWarps;
+  static constexpr int kThreads = 64 + 32 * (kEpiWarps + (FUSE ? kGQuantWarps + 1 : 0));
+  static constexpr uint32_t kRawRing = FUSE ? kGRawStages * kGRawBytes : 0;
   static constexpr uint32_t kTail = kEpiWarps * 64 * 4 + 512;  // bias, barriers, TMEM slot
-  static constexpr int kStages = (232448 - 1024 - kTail - kEpiWarps * kPanelBytes) / kStageBytes;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kEpiWarps * kPanelBytes + kTail;
+  static constexpr int kStages = (232448 - 1024 - kTail - kEpiWarps * kPanelBytes - kRawRing) / kStageBytes;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kEpiWarps * kPanelBytes + kRawRing + kTail;
   static constexpr uint32_t kSfCols = 8 + 8 * kBTiles;        // TMEM columns of one stage's scales
   static constexpr uint32_t kTmemCols = 2 * BN + 2 * kSfCols <= 256 ? 256 : 512;
   static_assert(2 * BN + 2 * kSfCols <= 512 && kStages >= 3, "tile does not fit");
-  static_assert((2 * kStages + 5 + kEpiWarps) * 8 + 4 <= 512, "barriers do not fit");
+  static_assert(!FUSE || kGBM == 2 * 4 * kGQuantWarps, "two passes of four rows a warp");
+  static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 4 <= 512, "barriers do not fit");
 };
 
 struct GemmMx4Dev {
@@ -238,22 +254,23 @@ struct GemmMx4Dev {
   int* err;
 };
 
-template <int BN, typename T, int ACT>
-__global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
+template <int BN, typename T, int ACT, bool FUSE>
+__global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
                     const GemmMx4Dev p) {
   constexpr bool GEGLU = ACT == 2;
-  using C = GCfg<BN, GEGLU>;
+  using C = GCfg<BN, GEGLU, FUSE>;
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sPanel = smem + S * (C::kABytes + C::kBBytes);
+  uint8_t* sRaw = smem + S * (C::kABytes + C::kBBytes);
+  uint8_t* sPanel = sRaw + C::kRawRing;
   uint8_t* sSf = sPanel + C::kEpiWarps * C::kPanelBytes;
   float* sBias = reinterpret_cast<float*>(sSf + S * C::kSfBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sBias + C::kEpiWarps * 64);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + C::kEpiWarps);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + C::kEpiWarps + 2 * kGRawStages);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
@@ -261,6 +278,8 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
   auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
   const uint32_t drain_bar = bar0 + 8u * (2 * S + 4);
   auto res_bar = [&](int w) { return bar0 + 8u * (2 * S + 5 + w); };
+  auto rfull_bar = [&](int s) { return bar0 + 8u * (2 * S + 5 + C::kEpiWarps + s); };
+  auto rempty_bar = [&](int s) { return bar0 + 8u * (2 * S + 5 + C::kEpiWarps + kGRawStages + s); };
 
   const int num_m = (p.M + kGBM - 1) / kGBM, num_n = (p.N + BN - 1) / BN;
   const long long num_tiles = (long long)num_m * num_n;
@@ -269,7 +288,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), FUSE ? 1 + kGQuantWarps : 1);
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -278,6 +297,11 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
     }
     mbar_init(drain_bar, 1);
     for (int w = 0; w < C::kEpiWarps; ++w) mbar_init(res_bar(w), 1);
+    if (FUSE)
+      for (int s = 0; s < kGRawStages; ++s) {
+        mbar_init(rfull_bar(s), 1);
+        mbar_init(rempty_bar(s), kGQuantWarps);
+      }
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -298,63 +322,77 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
   // 163 us with one after the last MMA, 161 us without; 8192 x 320 x 320 9.3 / 8.3 / 7.8 us.
 
   if (warp == 0) {
-    if (lane == 0) {
-      pdl_wait();
-      uint32_t it = 0;
-      bool ok = true;
-      for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const int m0 = (int)(tile / num_n) * kGBM, n0 = (int)(tile % num_n) * BN;
-        const uint8_t* xs = p.xs + (size_t)(m0 / kMxTileRows) * kts * kMxTileBytes;
-        const uint8_t* ws = p.ws + (size_t)(n0 / kMxTileRows) * kts * kMxTileBytes;
-        for (int k = 0; k < nst; ++k, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty)) { ok = false; break; }
-          const uint32_t sfb = (uint32_t)min(2, kts - 2 * k) * kMxTileBytes;  // scale bytes per 128 rows
-          int wt = 0;  // scale tiles of w that exist below row N (a tile behind N multiplies columns never stored)
-          for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
-          mbar_arrive_expect_tx(full_bar(s), C::kABytes + C::kBBytes + sfb * (1 + wt));
-          const uint32_t dA = smem_u32(smem + s * C::kABytes);
-          const uint32_t dB = smem_u32(smem + S * C::kABytes + s * C::kBBytes);
-          const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
-          tma_load_2d(dA, &map_x, full_bar(s), k * 128, m0);
-          tma_load_2d(dB, &map_w, full_bar(s), k * 128, n0);
-          bulk_load(dS, xs + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
-          for (int j = 0; j < wt; ++j)
-            bulk_load(dS + (1 + j) * 2 * kMxTileBytes, ws + ((size_t)j * kts + k * 2) * kMxTileBytes, sfb, full_bar(s));
-        }
-      }
-      // abort: every copy in flight lands before the shared memory is released
-      if (!ok)
-        for (uint32_t q = it > (uint32_t)S ? it - S : 0; q < it; ++q)
-          mbar_drain(full_bar(q % S), (q / S) & 1u, p.err, kDevTimeoutDrain);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t it = 0, tl = 0;
-      bool ok = true;
-      for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++tl) {
-        const int n0 = (int)(tile % num_n) * BN;
-        const uint32_t acc = tl & 1u;
-        if (!mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u, p.err, kDevTimeoutAcc)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        const uint32_t n_off = (uint32_t)(n0 % kMxTileRows) / 32u;  // BN = 64: the tile's half of its scale tile
-        for (int k = 0; k < nst; ++k, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(full_bar(s), (it / S) & 1u, p.err, kDevTimeoutFull)) { ok = false; break; }
-          const uint32_t sf = tmem_base + 2 * BN + (it & 1u) * C::kSfCols;
-          const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
-          const int cols = min(kGStageCols, kp - k * kGStageCols);
-          const int nkt = (cols + kMxTileCols - 1) / kMxTileCols;
-          for (int t = 0; t < nkt; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: 4 columns per tile, per 128 of K]
-            tmem_copy_scales(sf + 4 * t, sdesc_scales(dS + t * kMxTileBytes));
-#pragma unroll
-            for (int j = 0; j < C::kBTiles; ++j)
-              tmem_copy_scales(sf + 8 + 4 * (t * C::kBTiles + j), sdesc_scales(dS + (2 * (1 + j) + t) * kMxTileBytes));
+    // all lanes walk the loop and wait; one of them issues
+    pdl_wait();
+    uint32_t it = 0;
+    bool ok = true;
+    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int m0 = (int)(tile / num_n) * kGBM, n0 = (int)(tile % num_n) * BN;
+      const uint8_t* xs = FUSE ? nullptr : p.xs + (size_t)(m0 / kMxTileRows) * kts * kMxTileBytes;
+      const uint8_t* ws = p.ws + (size_t)(n0 / kMxTileRows) * kts * kMxTileBytes;
+      int wt = 0;  // scale tiles of w that exist below row N (a tile behind N multiplies columns never stored)
+      for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
+      for (int k = 0; k < nst; ++k, ++it) {
+        const int s = it % S;
+        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        if (!ok) break;
+        const uint32_t sfb = (uint32_t)min(2, kts - 2 * k) * kMxTileBytes;  // scale bytes per 128 rows
+        const uint32_t dA = smem_u32(smem + s * C::kABytes);
+        const uint32_t dB = smem_u32(smem + S * C::kABytes + s * C::kBBytes);
+        const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full_bar(s), FUSE ? C::kBBytes + sfb * wt : C::kABytes + C::kBBytes + sfb * (1 + wt));
+          if constexpr (!FUSE) {
+            tma_load_2d(dA, &map_x, full_bar(s), k * 128, m0);
+            bulk_load(dS, xs + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
           }
-          const uint64_t da = sdesc_sw128(smem_u32(smem + s * C::kABytes), 16, 1024);
-          const uint64_t db = sdesc_sw128(smem_u32(smem + S * C::kABytes + s * C::kBBytes), 16, 1024);
-          const int nmma = (cols + 63) / 64;
+          tma_load_2d(dB, &map_w, full_bar(s), k * 128, n0);
+#pragma unroll
+          for (int j = 0; j < C::kBTiles; ++j)
+            if (j < wt)
+              bulk_load(dS + (1 + j) * 2 * kMxTileBytes, ws + ((size_t)j * kts + k * 2) * kMxTileBytes, sfb, full_bar(s));
+        }
+        __syncwarp();
+      }
+    }
+    // abort: every copy in flight lands before the shared memory is released
+    if (!ok && lane == 0)
+      for (uint32_t q = it > (uint32_t)S ? it - S : 0; q < it; ++q)
+        mbar_drain(full_bar(q % S), (q / S) & 1u, p.err, kDevTimeoutDrain);
+  } else if (warp == 1) {
+    // all lanes walk the loop and wait; one of them issues
+    uint32_t it = 0, tl = 0;
+    bool ok = true;
+    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++tl) {
+      const int n0 = (int)(tile % num_n) * BN;
+      const uint32_t acc = tl & 1u;
+      ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u, p.err, kDevTimeoutAcc));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + acc * BN;
+      const uint32_t n_off = (uint32_t)(n0 % kMxTileRows) / 32u;  // BN = 64: the tile's half of its scale tile
+      for (int k = 0; k < nst; ++k, ++it) {
+        const int s = it % S;
+        ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (it / S) & 1u, p.err, kDevTimeoutFull));
+        if (!ok) break;
+        const uint32_t sf = tmem_base + 2 * BN + (it & 1u) * C::kSfCols;
+        const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
+        const int cols = min(kGStageCols, kp - k * kGStageCols);
+        const int nkt = (cols + kMxTileCols - 1) / kMxTileCols;
+        const uint64_t ds = sdesc_scales(dS);
+        const uint64_t da = sdesc_sw128(smem_u32(smem + s * C::kABytes), 16, 1024);
+        const uint64_t db = sdesc_sw128(smem_u32(smem + S * C::kABytes + s * C::kBBytes), 16, 1024);
+        const int nmma = (cols + 63) / 64;
+        if (elect_one()) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: 4 columns per tile, per 128 of K]
+            if (t < nkt) {
+              tmem_copy_scales(sf + 4 * t, ds + (t * kMxTileBytes >> 4));
+#pragma unroll
+              for (int j = 0; j < C::kBTiles; ++j)
+                tmem_copy_scales(sf + 8 + 4 * (t * C::kBTiles + j), ds + ((2 * (1 + j) + t) * kMxTileBytes >> 4));
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (j < nmma)
@@ -362,11 +400,94 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
                           sf + 8 + 4 * (j >> 1) * C::kBTiles + n_off, (k | j) != 0);
           mma_commit(empty_bar(s));
         }
-        if (!ok) break;
-        mma_commit(tfull_bar(acc));
+        __syncwarp();
       }
-      mma_commit(drain_bar);  // every issued copy and MMA has retired before TMEM is released
-      mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain);
+      if (!ok) break;
+      if (elect_one()) mma_commit(tfull_bar(acc));
+      __syncwarp();
+    }
+    if (elect_one()) mma_commit(drain_bar);  // every issued copy and MMA has retired before TMEM is released
+    __syncwarp();
+    if (lane == 0) mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain);
+  } else if (FUSE && warp == 2 + C::kEpiWarps + kGQuantWarps) {
+    // x into the raw ring
+    pdl_wait();
+    const int nraw = (kp + 127) / 128;
+    uint32_t it = 0;
+    bool ok = true;
+    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int m0 = (int)(tile / num_n) * kGBM;
+      for (int k = 0; k < nraw; ++k, ++it) {
+        const int s = it % kGRawStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        if (!ok) break;
+        const uint32_t d = smem_u32(sRaw + s * kGRawBytes);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(rfull_bar(s), kGRawBytes);
+          tma_load_2d(d, &map_x, rfull_bar(s), k * 128, m0);
+          tma_load_2d(d + kGRawBytes / 2, &map_x, rfull_bar(s), k * 128 + 64, m0);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0)
+      for (uint32_t q = it > (uint32_t)kGRawStages ? it - kGRawStages : 0; q < it; ++q)
+        mbar_drain(rfull_bar(q % kGRawStages), (q / kGRawStages) & 1u, p.err, kDevTimeoutDrain);
+  } else if (FUSE && warp >= 2 + C::kEpiWarps) {
+    // quantiser: four rows a pass and warp (64 a pass in all), eight lanes a row, 16 columns a lane
+    const int l = lane & 7, r0 = (warp - 2 - C::kEpiWarps) * 4 + (lane >> 3);
+    uint32_t it = 0, rit = 0;
+    bool ok = true;
+    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      for (int k = 0; k < nst && ok; ++k, ++it) {
+        const int s = it % S;
+        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        if (!ok) break;
+        uint8_t* dA = smem + s * C::kABytes;
+        uint8_t* dS = sSf + s * C::kSfBytes;
+        const int halves = kp - k * kGStageCols > 128 ? 2 : 1;
+        for (int h = 0; h < halves; ++h, ++rit) {
+          const int rs = rit % kGRawStages;
+          ok = __all_sync(0xffffffffu, mbar_wait(rfull_bar(rs), (rit / kGRawStages) & 1u, p.err, kDevTimeoutFull));
+          if (!ok) break;
+          // 64-column box l / 4; its 16-byte chunks are XORed with the row as TMA wrote them
+          const uint8_t* src = sRaw + rs * kGRawBytes + (l >> 2) * (kGRawBytes / 2);
+          // both passes side by side: one alone is a chain of dependent steps (rows behind M are zero)
+          MxRaw<T> raw[2];
+          uint32_t e[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 64 * i;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + r * 128 + (((2 * (l & 3) + c) ^ (r & 7)) << 4));
+              raw[i].w[4 * c] = u.x; raw[i].w[4 * c + 1] = u.y; raw[i].w[4 * c + 2] = u.z; raw[i].w[4 * c + 3] = u.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) e[i] = mx_raw_amax<T>(raw[i]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) e[i] = mx_exponent(mx_block_amax<T>(e[i]));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 64 * i;
+            float v[16];
+            mx_unpack<T>(raw[i], v);
+            uint32_t q[2];
+            mx_codes<16>(v, e[i], q);
+            // codes in the 128 B-swizzled layout that TMA would have written; scales in their tile's order
+            *reinterpret_cast<uint2*>(dA + r * 128 + (((4 * h + (l >> 1)) ^ (r & 7)) << 4) + (l & 1) * 8) =
+                make_uint2(q[0], q[1]);
+            if ((l & 1) == 0) dS[h * kMxTileBytes + mx_scale_byte(r, l >> 1)] = (uint8_t)e[i];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(rempty_bar(rs));
+        }
+        if (!ok) break;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(s));
+      }
     }
   } else {
     pdl_wait();
@@ -374,7 +495,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
     const int w = warp - 2, set = w / C::kSetWarps, lg = warp & 3, pn = (w % C::kSetWarps) >> 2;
     float* bias_s = sBias + w * 64;
     uint8_t* pan = sPanel + w * C::kPanelBytes;
-    const long long tstep = 2ll * gridDim.x;
+    const long long tstep = (long long)C::kSets * gridDim.x;
     auto load_res = [&](long long tile) {  // lane 0
       mbar_arrive_expect_tx(res_bar(w), C::kPanelBytes);
       tma_load_2d(smem_u32(pan), &map_r, res_bar(w), (int)(tile % num_n) * BN + pn * 64,
@@ -392,14 +513,15 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
       bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? p.bias[n + 32 + lane] : 0.f;
       if (!p.residual && lane == 0) bulk_wait_read<0>();  // the panel's previous store has read it
       __syncwarp();
-      bool ok = mbar_wait(tfull_bar(set), q & 1u, p.err, kDevTimeoutAcc);
+      const uint32_t tl = q * C::kSets + set, acc = tl & 1u;  // the block's tile number, and its accumulator
+      bool ok = mbar_wait(tfull_bar(acc), (tl >> 1) & 1u, p.err, kDevTimeoutAcc);
       if (ok && p.residual) {
         ok = mbar_wait(res_bar(w), q & 1u, p.err, kDevTimeoutEmpty);
         if (ok) loading = false;
       }
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + set * BN + pn * 64 + (static_cast<uint32_t>(lg * 32) << 16);
+      const uint32_t t_row = tmem_base + acc * BN + pn * 64 + (static_cast<uint32_t>(lg * 32) << 16);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t r[32];
@@ -408,7 +530,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
         if (h == 1) {  // the accumulator's last read of this warp
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty_bar(set));
+          if (lane == 0) mbar_arrive(tempty_bar(acc));
         }
         const float4* b4 = reinterpret_cast<const float4*>(bias_s + 32 * h);
         auto acc2 = [&](int i, float x, float y) {
@@ -479,10 +601,10 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2>::kThreads, 1)
   }
 }
 
-template <int BN, typename T, int ACT>
+template <int BN, typename T, int ACT, bool FUSE>
 cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  using C = GCfg<BN, ACT == 2>;
-  auto k = mx4_gemm_kernel<BN, T, ACT>;
+  using C = GCfg<BN, ACT == 2, FUSE>;
+  auto k = mx4_gemm_kernel<BN, T, ACT, FUSE>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -506,9 +628,17 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
     return make_tmap(m, base, 2, dims, str, box, C::kPW == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                      CU_TENSOR_MAP_DATA_TYPE_UINT16);
   };
-  if (!codes(&mx, a.xcodes, a.M, kGBM) || !codes(&mw, a.wcodes, a.N, BN) || !panel(&my, a.y) ||
-      !panel(&mr, a.residual ? a.residual : a.y))
-    return cudaErrorInvalidValue;
+  if (!codes(&mw, a.wcodes, a.N, BN) || !panel(&my, a.y)) return cudaErrorInvalidValue;
+  mr = my;
+  if (a.residual && !panel(&mr, a.residual)) return cudaErrorInvalidValue;
+  if constexpr (FUSE) {
+    const uint64_t dims[2] = {(uint64_t)a.K, (uint64_t)a.M}, str[1] = {(uint64_t)a.ldx * 2};
+    const uint32_t box[2] = {64, kGBM};
+    if (!make_tmap(&mx, a.x, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_UINT16))
+      return cudaErrorInvalidValue;
+  } else {
+    if (!codes(&mx, a.xcodes, a.M, kGBM)) return cudaErrorInvalidValue;
+  }
   GemmMx4Dev p;
   p.M = a.M; p.N = a.N; p.K = a.K;
   p.xs = a.xscales; p.ws = a.wscales; p.bias = a.bias; p.residual = a.residual != nullptr; p.err = err;
@@ -520,13 +650,22 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 template <typename T, int ACT>
 cudaError_t gemm_bn(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + 127) / 128);
-  if (tiles >= num_sms()) return launch_gemm_mx4<128, T, ACT>(a, err, s);
-  return launch_gemm_mx4<64, T, ACT>(a, err, s);
+  if (a.x) return launch_gemm_mx4<64, T, ACT, true>(a, err, s);
+  return tiles >= num_sms() ? launch_gemm_mx4<128, T, ACT, false>(a, err, s) : launch_gemm_mx4<64, T, ACT, false>(a, err, s);
 }
+
+// The fused form while a block quantises at most this many stages (256 columns of 128 rows, about 1.3 us each). Measured
+// on B200, fused against quantise + product: one eager call 12.3 against 16.4 us (the second launch and the scratch's
+// allocation cost the host 4 us), the device alone 154 x 2560 x 768 7.9 / 5.2 us, 8192 x 320 x 320 10.9 / 7.2 us; beyond
+// six stages the device time passes the host's.
+constexpr long long kFuseStages = 6;
+
+// Few rows run on the CUDA cores, as long as their operand fits 48 KB of shared memory.
+bool linear_rows(int M, int K) { return M <= 8 && (size_t)8 * (mx_kp(K) / 2 + mx_kp(K) / 8) <= 48 * 1024; }
 
 template <typename T>
 cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  if (mx4_linear_rows(a.M, a.K)) {
+  if (linear_rows(a.M, a.K)) {
     return a.M == 1 ? launch_rows<T, 1>(a, s) : a.M == 2 ? launch_rows<T, 2>(a, s) : a.M <= 4 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
   }
   switch (a.act) {
@@ -538,8 +677,14 @@ cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 
 }  // namespace
 
-// Few rows run on the CUDA cores, as long as their operand fits 48 KB of shared memory.
-bool mx4_linear_rows(int M, int K) { return M <= 8 && (size_t)8 * (mx_kp(K) / 2 + mx_kp(K) / 8) <= 48 * 1024; }
+bool mx4_linear_takes_x(const void* x, int M, int K, long long ldx, int N) {
+  if (linear_rows(M, K)) return true;
+  // the fused form reads x by TMA: aligned rows, a stride that a tensor map can hold
+  const bool tma = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && ldx >= K;
+  if (!tma) return false;
+  const long long tiles = (long long)((M + kGBM - 1) / kGBM) * ((N + 63) / 64), rounds = (tiles + num_sms() - 1) / num_sms();
+  return rounds * ((mx_kp(K) + kGStageCols - 1) / kGStageCols) <= kFuseStages;
+}
 
 cudaError_t launch_mx4_linear(const Mx4LinearArgs& a, int* dev_err, cudaStream_t s) {
   return a.dtype == kBF16 ? linear_t<__nv_bfloat16>(a, dev_err, s) : linear_t<__half>(a, dev_err, s);

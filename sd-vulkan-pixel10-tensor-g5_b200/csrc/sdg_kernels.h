@@ -138,7 +138,7 @@ cudaError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
 // y = act(x w^T + bias + residual): x [M, K], w [N, K] MXFP4, y [M, N] (act 2, GEGLU: [M, N/2], w rows and bias
 // interleaved 16 value / 16 gate as for kEpiGeglu); residual and y of type dtype (kF16 or kBF16).
 struct Mx4LinearArgs {
-  const void* x = nullptr; long long ldx = 0;  // a plain x of type dtype: only where mx4_linear_rows(M, K)
+  const void* x = nullptr; long long ldx = 0;  // a plain x of type dtype: only where mx4_linear_takes_x
   const uint8_t* xcodes = nullptr; const uint8_t* xscales = nullptr;
   const uint8_t* wcodes = nullptr; const uint8_t* wscales = nullptr;
   int M = 0, N = 0, K = 0;
@@ -146,8 +146,8 @@ struct Mx4LinearArgs {
   int act = 0, dtype = kF16;
   void* y = nullptr;
 };
-// Whether the product takes a plain x itself (few rows); otherwise it wants the operand.
-bool mx4_linear_rows(int M, int K);
+// Whether the product quantises a plain x itself (few rows, small products); otherwise it wants the operand.
+bool mx4_linear_takes_x(const void* x, int M, int K, long long ldx, int N);
 cudaError_t launch_mx4_linear(const Mx4LinearArgs& a, int* dev_err, cudaStream_t s);
 // GroupNorm (+ SiLU) of channels-last x [B, HW, C] (kF16 or kBF16) -> operand [B * HW, C]. stats:
 // mx4_groupnorm_scratch_bytes() bytes.

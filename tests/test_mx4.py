@@ -78,9 +78,11 @@ def test_sizes(sdg):
     assert L.sdg_mx4_code_bytes(3, 33) == 3 * 32 and L.sdg_mx4_scale_bytes(3, 33) == 512
     assert L.sdg_mx4_code_bytes(129, 320) == 129 * 160 and L.sdg_mx4_scale_bytes(129, 320) == 2 * 3 * 512
     assert L.sdg_mx4_code_bytes(0, 5) == 0 and L.sdg_mx4_scale_bytes(5, -1) == 0
-    assert L.sdg_linear_mx4_scratch_bytes(3, 33) == 0                # few rows: no scratch
-    assert L.sdg_linear_mx4_scratch_bytes(9, 33) == 512 + 512
-    assert L.sdg_linear_mx4_scratch_bytes(300, 320) == 300 * 160 + 128 + 3 * 3 * 512
+    need = L.sdg_linear_mx4_scratch_bytes
+    assert need(16, 3, 33, 33, 64) == 0 and need(16, 100, 320, 320, 64) == 0   # few rows, small products: no scratch
+    assert need(18, 100, 320, 320, 64) == need(16, 100, 320, 323, 64) == 100 * 160 + 384 + 3 * 512  # unaligned rows
+    assert need(16, 0, 33, 33, 64) == 0
+    assert need(16, 100001, 320, 320, 1280) == 100001 * 160 + 352 + 782 * 3 * 512
 
 
 def _addr(n=4096):
@@ -104,10 +106,10 @@ def test_refusals_without_gpu(sdg):
     assert m(M=0) == m(K=0) == m(N=0) == m(act=3) == m(act=-1) == m(dt=2) == SDG_ERR_ARG
     assert m(act=2, r=p) == m(xc=p + 8) == m(wc=p + 8) == m(y=p + 2) == m(r=p + 2) == m(b=p + 2) == SDG_ERR_ARG
     assert m(N=12) == m(N=40, act=2) == SDG_ERR_SHAPE
-    bx = {"x": p, "M": 9, "K": 32, "ld": 32, "wc": p, "ws": p, "b": None, "N": 32, "r": None, "act": 0, "dt": 0, "y": p,
-          "scr": p, "nb": 1024, "err": None, "st": None}
+    bx = {"x": p, "M": 1 << 20, "K": 32, "ld": 32, "wc": p, "ws": p, "b": None, "N": 32, "r": None, "act": 0, "dt": 0, "y": p,
+          "scr": p, "nb": 1 << 30, "err": None, "st": None}
     mx = lambda **k: L.sdg_linear_mx4_x(*(bx | k).values())
-    assert mx(x=None) == mx(scr=None) == mx(nb=1023) == mx(scr=p + 8) == mx(ld=-2) == mx(dt=2) == SDG_ERR_ARG
+    assert mx(x=None) == mx(scr=None) == mx(nb=1 << 24) == mx(scr=p + 8) == mx(ld=-2) == mx(dt=2) == SDG_ERR_ARG
     g = lambda **k: L.sdg_groupnorm_mx4(*({"x": p, "dt": 0, "B": 1, "HW": 4, "C": 64, "G": 8, "ga": p, "be": p, "eps": 1e-5,
                                            "silu": 0, "c": p, "s": p, "scr": p, "st": None} | k).values())
     assert g(x=None) == g(ga=None) == g(c=None) == g(scr=None) == g(B=0) == g(HW=0) == g(C=0) == g(G=0) == SDG_ERR_ARG
