@@ -209,6 +209,9 @@ cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
 //               takes 32 rows x 64 accumulator columns through a swizzled shared-memory panel that TMA fills with the
 //               residual beforehand and stores from afterwards, so global memory is only touched in full lines
 // Accumulators are double-buffered in TMEM, one per set.
+// PAIR: two CTAs on two SMs compute 256 x BN with tcgen05.mma.cta_group::2, each with its 128 rows of x and half the rows
+// of w: a quarter fewer bytes into and out of shared memory per product, six stages instead of four, but two CTAs
+// to synchronise per tile. It pays for long rows only (both sides at kPairStages below).
 // FUSE (BN = 64): x is quantised on the way, so the call is one launch without scratch: one more warp brings tiles of
 // 128 rows x 128 columns of x into a ring by TMA and sixteen more quantise them into the code stages. (Loading x into
 // registers a stage ahead instead ran four times slower: the loads in flight share the scoreboard that the pass in
@@ -222,15 +225,17 @@ constexpr int kGQuantWarps = 16;
 constexpr int kGRawStages = 3;
 constexpr uint32_t kGRawBytes = kGBM * 128 * 2;  // 128 columns of 16 bits, as two 128 B-swizzled boxes of 64
 
-template <int BN, bool GEGLU, bool FUSE>
+template <int BN, bool GEGLU, bool FUSE, bool PAIR>
 struct GCfg {
   static constexpr int kBTiles = (BN + kMxTileRows - 1) / kMxTileRows;  // scale tiles of w per 128 columns of K
-  static constexpr uint32_t kABytes = kGBM * 128, kBBytes = BN * 128;
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of w in this CTA
+  static constexpr uint32_t kABytes = kGBM * 128, kBBytes = kBRows * 128;
   static constexpr uint32_t kSfBytes = 2 * kMxTileBytes * (1 + kBTiles);
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr int kPW = GEGLU ? 32 : 64;                 // output columns of a panel (64 accumulator columns)
   static constexpr uint32_t kPanelBytes = 32 * kPW * 2;
   static_assert(!FUSE || BN == 64, "the fused form has 64-wide tiles");
+  static_assert(!PAIR || (BN == 128 && !FUSE), "pairs have 128-wide tiles");
   static constexpr int kSets = FUSE ? 1 : 2;
   static constexpr int kSetWarps = 4 * (BN / 64), kEpiWarps = kSets * kSetWarps;
   static constexpr int kThreads = 64 + 32 * (kEpiWarps + (FUSE ? kGQuantWarps + 1 : 0));
@@ -245,6 +250,27 @@ struct GCfg {
   static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 4 <= 512, "barriers do not fit");
 };
 
+// A block's walk over the tiles first, first + step, ... (n fastest), without a division per tile.
+struct TileWalk {
+  int m, n;  // tile coordinates
+  int dm, dn, num_m, num_n;
+  __device__ TileWalk(int first, int step, int num_m_, int num_n_) : num_m(num_m_), num_n(num_n_) {
+    m = first / num_n;
+    n = first - m * num_n;
+    dm = step / num_n;
+    dn = step - dm * num_n;
+  }
+  __device__ __forceinline__ bool valid() const { return m < num_m; }
+  __device__ __forceinline__ void next() {
+    m += dm;
+    n += dn;
+    if (n >= num_n) {
+      n -= num_n;
+      ++m;
+    }
+  }
+};
+
 struct GemmMx4Dev {
   int M, N, K;
   const uint8_t* xs;
@@ -254,13 +280,15 @@ struct GemmMx4Dev {
   int* err;
 };
 
-template <int BN, typename T, int ACT, bool FUSE>
-__global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
+template <int BN, typename T, int ACT, bool FUSE, bool PAIR>
+__global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
+                    const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws,
                     const GemmMx4Dev p) {
   constexpr bool GEGLU = ACT == 2;
-  using C = GCfg<BN, GEGLU, FUSE>;
+  using C = GCfg<BN, GEGLU, FUSE, PAIR>;
+  constexpr int TM = PAIR ? 2 * kGBM : kGBM;  // rows of a tile
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -281,8 +309,9 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
   auto rfull_bar = [&](int s) { return bar0 + 8u * (2 * S + 5 + C::kEpiWarps + s); };
   auto rempty_bar = [&](int s) { return bar0 + 8u * (2 * S + 5 + C::kEpiWarps + kGRawStages + s); };
 
-  const int num_m = (p.M + kGBM - 1) / kGBM, num_n = (p.N + BN - 1) / BN;
-  const long long num_tiles = (long long)num_m * num_n;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int team = PAIR ? blockIdx.x >> 1 : blockIdx.x, teams = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + BN - 1) / BN;
   const int kp = mx_kp(p.K), kts = mx_ktiles(p.K);
   const int nst = (kp + kGStageCols - 1) / kGStageCols;  // stages per tile
 
@@ -293,7 +322,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), C::kSetWarps);
+      mbar_init(tempty_bar(a), C::kSetWarps * (PAIR ? 2 : 1));  // a pair's warps arrive at the even CTA's
     }
     mbar_init(drain_bar, 1);
     for (int w = 0; w < C::kEpiWarps; ++w) mbar_init(res_bar(w), 1);
@@ -310,11 +339,20 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     tma_prefetch_desc(&map_y);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc2(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish2();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  if constexpr (PAIR)
+    cluster_sync_all();  // both CTAs' barriers and TMEM stand before any signal crosses
+  else
+    __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // No early trigger: blocks of the next kernel that move in while this one runs hold their SMs' warps and registers
@@ -326,10 +364,17 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     pdl_wait();
     uint32_t it = 0;
     bool ok = true;
-    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const int m0 = (int)(tile / num_n) * kGBM, n0 = (int)(tile % num_n) * BN;
+    for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
+      const int m0 = tw.m * TM + rank * kGBM, n0 = tw.n * BN;
       const uint8_t* xs = FUSE ? nullptr : p.xs + (size_t)(m0 / kMxTileRows) * kts * kMxTileBytes;
       const uint8_t* ws = p.ws + (size_t)(n0 / kMxTileRows) * kts * kMxTileBytes;
+      // The x tile of this block's next round into L2, by the one block whose next tile is the first of its row, where the
+      // rows are long: the ring holds too little to cover HBM's latency (65536 x 640 x 2560 72 -> 66 us; at K <= 1024 the
+      // extra requests cost more than they hide)
+      TileWalk tn = tw;
+      tn.next();
+      const bool ahead = !FUSE && nst > 4 && tn.valid() && tn.n == 0;
+      const int m1 = tn.m * TM + rank * kGBM;
       int wt = 0;  // scale tiles of w that exist below row N (a tile behind N multiplies columns never stored)
       for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
       for (int k = 0; k < nst; ++k, ++it) {
@@ -341,82 +386,114 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
         const uint32_t dB = smem_u32(smem + S * C::kABytes + s * C::kBBytes);
         const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
         if (elect_one()) {
-          mbar_arrive_expect_tx(full_bar(s), FUSE ? C::kBBytes + sfb * wt : C::kABytes + C::kBBytes + sfb * (1 + wt));
-          if constexpr (!FUSE) {
-            tma_load_2d(dA, &map_x, full_bar(s), k * 128, m0);
-            bulk_load(dS, xs + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
-          }
-          tma_load_2d(dB, &map_w, full_bar(s), k * 128, n0);
+          if (ahead) tma_prefetch_2d(&map_x, k * 128, m1);
+          if constexpr (PAIR) {
+            // both CTAs' bytes count on the even CTA's barrier; scale tiles come through tensor maps (zero behind the last)
+            if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * C::kStageBytes);
+            const uint32_t fb = mapa_shared(full_bar(s), 0);
+            tma_load_2d_pair(dA, &map_x, fb, k * 128, m0);
+            tma_load_2d_pair(dS, &map_xs, fb, k * 256, m0 / kMxTileRows);
+            tma_load_2d_pair(dB, &map_w, fb, k * 128, n0 + rank * C::kBRows);
+            tma_load_2d_pair(dS + 2 * kMxTileBytes, &map_ws, fb, k * 256, n0 / kMxTileRows);
+          } else {
+            mbar_arrive_expect_tx(full_bar(s), FUSE ? C::kBBytes + sfb * wt : C::kABytes + C::kBBytes + sfb * (1 + wt));
+            if constexpr (!FUSE) {
+              tma_load_2d(dA, &map_x, full_bar(s), k * 128, m0);
+              bulk_load(dS, xs + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
+            }
+            tma_load_2d(dB, &map_w, full_bar(s), k * 128, n0);
 #pragma unroll
-          for (int j = 0; j < C::kBTiles; ++j)
-            if (j < wt)
-              bulk_load(dS + (1 + j) * 2 * kMxTileBytes, ws + ((size_t)j * kts + k * 2) * kMxTileBytes, sfb, full_bar(s));
+            for (int j = 0; j < C::kBTiles; ++j)
+              if (j < wt)
+                bulk_load(dS + (1 + j) * 2 * kMxTileBytes, ws + ((size_t)j * kts + k * 2) * kMxTileBytes, sfb, full_bar(s));
+          }
         }
         __syncwarp();
       }
     }
     // abort: every copy in flight lands before the shared memory is released
-    if (!ok && lane == 0)
-      for (uint32_t q = it > (uint32_t)S ? it - S : 0; q < it; ++q)
-        mbar_drain(full_bar(q % S), (q / S) & 1u, p.err, kDevTimeoutDrain);
+    if (!ok && lane == 0) {
+      if (rank == 0) {
+        for (uint32_t q = it > (uint32_t)S ? it - S : 0; q < it; ++q)
+          mbar_drain(full_bar(q % S), (q / S) & 1u, p.err, kDevTimeoutDrain);
+      } else {
+        spin_ns(200000);  // the odd CTA cannot see the even CTA's barriers
+      }
+    }
   } else if (warp == 1) {
-    // all lanes walk the loop and wait; one of them issues
-    uint32_t it = 0, tl = 0;
-    bool ok = true;
-    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++tl) {
-      const int n0 = (int)(tile % num_n) * BN;
-      const uint32_t acc = tl & 1u;
-      ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u, p.err, kDevTimeoutAcc));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + acc * BN;
-      const uint32_t n_off = (uint32_t)(n0 % kMxTileRows) / 32u;  // BN = 64: the tile's half of its scale tile
-      for (int k = 0; k < nst; ++k, ++it) {
-        const int s = it % S;
-        ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (it / S) & 1u, p.err, kDevTimeoutFull));
+    if (rank == 0) {
+      // all lanes walk the loop and wait; one of them issues
+      auto copy_scales = [](uint32_t d, uint64_t s) {
+        if constexpr (PAIR) tmem_copy_scales2(d, s); else tmem_copy_scales(d, s);
+      };
+      auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+        if constexpr (PAIR) mma_mxf4_ss2(d, a, b, id, sa, sb, accumulate); else mma_mxf4_ss(d, a, b, id, sa, sb, accumulate);
+      };
+      auto commit = [](uint32_t bar) {  // a pair's signal goes to both CTAs
+        if constexpr (PAIR) mma_commit2_mc(bar, 0x3); else mma_commit(bar);
+      };
+      uint32_t it = 0, tl = 0;
+      bool ok = true;
+      for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next(), ++tl) {
+        const int n0 = tw.n * BN;
+        const uint32_t acc = tl & 1u;
+        const uint32_t free_ph = ((tl >> 1) & 1u) ^ 1u;
+        ok = __all_sync(0xffffffffu, PAIR ? mbar_wait_cluster(tempty_bar(acc), free_ph, p.err, kDevTimeoutAcc)
+                                          : mbar_wait(tempty_bar(acc), free_ph, p.err, kDevTimeoutAcc));
         if (!ok) break;
-        const uint32_t sf = tmem_base + 2 * BN + (it & 1u) * C::kSfCols;
-        const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
-        const int cols = min(kGStageCols, kp - k * kGStageCols);
-        const int nkt = (cols + kMxTileCols - 1) / kMxTileCols;
-        const uint64_t ds = sdesc_scales(dS);
-        const uint64_t da = sdesc_sw128(smem_u32(smem + s * C::kABytes), 16, 1024);
-        const uint64_t db = sdesc_sw128(smem_u32(smem + S * C::kABytes + s * C::kBBytes), 16, 1024);
-        const int nmma = (cols + 63) / 64;
-        if (elect_one()) {
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        const uint32_t n_off = (uint32_t)(n0 % kMxTileRows) / 32u;  // BN = 64: the tile's half of its scale tile
+        for (int k = 0; k < nst; ++k, ++it) {
+          const int s = it % S;
+          ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (it / S) & 1u, p.err, kDevTimeoutFull));
+          if (!ok) break;
+          const uint32_t sf = tmem_base + 2 * BN + (it & 1u) * C::kSfCols;
+          const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
+          const int cols = min(kGStageCols, kp - k * kGStageCols);
+          const int nkt = (cols + kMxTileCols - 1) / kMxTileCols;
+          const uint64_t ds = sdesc_scales(dS);
+          const uint64_t da = sdesc_sw128(smem_u32(smem + s * C::kABytes), 16, 1024);
+          const uint64_t db = sdesc_sw128(smem_u32(smem + S * C::kABytes + s * C::kBBytes), 16, 1024);
+          const int nmma = (cols + 63) / 64;
+          if (elect_one()) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: 4 columns per tile, per 128 of K]
-            if (t < nkt) {
-              tmem_copy_scales(sf + 4 * t, ds + (t * kMxTileBytes >> 4));
+            for (int t = 0; t < 2; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: 4 columns per tile, per 128 of K]
+              if (t < nkt) {
+                copy_scales(sf + 4 * t, ds + (t * kMxTileBytes >> 4));
 #pragma unroll
-              for (int j = 0; j < C::kBTiles; ++j)
-                tmem_copy_scales(sf + 8 + 4 * (t * C::kBTiles + j), ds + ((2 * (1 + j) + t) * kMxTileBytes >> 4));
+                for (int j = 0; j < C::kBTiles; ++j)
+                  copy_scales(sf + 8 + 4 * (t * C::kBTiles + j), ds + ((2 * (1 + j) + t) * kMxTileBytes >> 4));
+              }
             }
-          }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < nmma)
-              mma_mxf4_ss(d_tmem, da + 2ull * j, db + 2ull * j, idesc_mxf4(kGBM, BN, (j & 1) * 2), sf + 4 * (j >> 1),
-                          sf + 8 + 4 * (j >> 1) * C::kBTiles + n_off, (k | j) != 0);
-          mma_commit(empty_bar(s));
+            for (int j = 0; j < 4; ++j)
+              if (j < nmma)
+                mma(d_tmem, da + 2ull * j, db + 2ull * j, idesc_mxf4(TM, BN, (j & 1) * 2), sf + 4 * (j >> 1),
+                    sf + 8 + 4 * (j >> 1) * C::kBTiles + n_off, (k | j) != 0);
+            commit(empty_bar(s));
+          }
+          __syncwarp();
         }
+        if (!ok) break;
+        if (elect_one()) commit(tfull_bar(acc));
         __syncwarp();
       }
-      if (!ok) break;
-      if (elect_one()) mma_commit(tfull_bar(acc));
+      if (elect_one()) {
+        if constexpr (PAIR) mma_commit2_mc(drain_bar, 0x1); else mma_commit(drain_bar);
+      }
+      // every issued copy and MMA has retired before TMEM is released
       __syncwarp();
+      if (lane == 0) mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain);
     }
-    if (elect_one()) mma_commit(drain_bar);  // every issued copy and MMA has retired before TMEM is released
-    __syncwarp();
-    if (lane == 0) mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain);
   } else if (FUSE && warp == 2 + C::kEpiWarps + kGQuantWarps) {
     // x into the raw ring
     pdl_wait();
     const int nraw = (kp + 127) / 128;
     uint32_t it = 0;
     bool ok = true;
-    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const int m0 = (int)(tile / num_n) * kGBM;
+    for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
+      const int m0 = tw.m * kGBM;
       for (int k = 0; k < nraw; ++k, ++it) {
         const int s = it % kGRawStages;
         ok = __all_sync(0xffffffffu, mbar_wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
@@ -438,7 +515,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     const int l = lane & 7, r0 = (warp - 2 - C::kEpiWarps) * 4 + (lane >> 3);
     uint32_t it = 0, rit = 0;
     bool ok = true;
-    for (long long tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+    for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
       for (int k = 0; k < nst && ok; ++k, ++it) {
         const int s = it % S;
         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
@@ -495,20 +572,19 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     const int w = warp - 2, set = w / C::kSetWarps, lg = warp & 3, pn = (w % C::kSetWarps) >> 2;
     float* bias_s = sBias + w * 64;
     uint8_t* pan = sPanel + w * C::kPanelBytes;
-    const long long tstep = (long long)C::kSets * gridDim.x;
-    auto load_res = [&](long long tile) {  // lane 0
+    auto load_res = [&](int tm, int tn) {  // lane 0
       mbar_arrive_expect_tx(res_bar(w), C::kPanelBytes);
-      tma_load_2d(smem_u32(pan), &map_r, res_bar(w), (int)(tile % num_n) * BN + pn * 64,
-                  (int)(tile / num_n) * kGBM + lg * 32);
+      tma_load_2d(smem_u32(pan), &map_r, res_bar(w), tn * BN + pn * 64, tm * TM + rank * kGBM + lg * 32);
     };
-    long long tile = blockIdx.x + (long long)set * gridDim.x;
+    TileWalk tw(team + set * teams, C::kSets * teams, num_m, num_n);
     bool loading = false;  // a residual copy of this warp is in flight (lane 0)
-    if (p.residual && lane == 0 && tile < num_tiles) {
-      load_res(tile);
+    if (p.residual && lane == 0 && tw.valid()) {
+      load_res(tw.m, tw.n);
       loading = true;
     }
-    for (uint32_t q = 0; tile < num_tiles; tile += tstep, ++q) {
-      const int m0 = (int)(tile / num_n) * kGBM, n = (int)(tile % num_n) * BN + pn * 64;
+    for (uint32_t q = 0; tw.valid(); ++q) {
+      const int m0 = tw.m * TM + rank * kGBM, n = tw.n * BN + pn * 64;
+      tw.next();  // from here on the next tile
       bias_s[lane] = p.bias && n + lane < p.N ? p.bias[n + lane] : 0.f;
       bias_s[32 + lane] = p.bias && n + 32 + lane < p.N ? p.bias[n + 32 + lane] : 0.f;
       if (!p.residual && lane == 0) bulk_wait_read<0>();  // the panel's previous store has read it
@@ -530,7 +606,12 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
         if (h == 1) {  // the accumulator's last read of this warp
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty_bar(acc));
+          if (lane == 0) {
+            if (PAIR && rank != 0)
+              mbar_arrive_cluster(mapa_shared(tempty_bar(acc), 0));
+            else
+              mbar_arrive(tempty_bar(acc));
+          }
         }
         const float4* b4 = reinterpret_cast<const float4*>(bias_s + 32 * h);
         auto acc2 = [&](int i, float x, float y) {
@@ -580,9 +661,9 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
       if (lane == 0) {
         tma_store_2d(&map_y, smem_u32(pan), GEGLU ? n / 2 : n, m0 + lg * 32);
         bulk_commit();
-        if (p.residual && tile + tstep < num_tiles) {  // the panel takes the next residual once the store has read it
+        if (p.residual && tw.valid()) {  // the panel takes the next residual once the store has read it
           bulk_wait_read<0>();
-          load_res(tile + tstep);
+          load_res(tw.m, tw.n);
           loading = true;
         }
       }
@@ -594,17 +675,25 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE>::kThreads, 1)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  if constexpr (PAIR)
+    cluster_sync_all();  // neither CTA frees TMEM or shared memory that the pair still uses
+  else
+    __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, C::kTmemCols);
+    if constexpr (PAIR)
+      tmem_dealloc2(tmem_base, C::kTmemCols);
+    else
+      tmem_dealloc(tmem_base, C::kTmemCols);
   }
 }
 
-template <int BN, typename T, int ACT, bool FUSE>
+template <int BN, typename T, int ACT, bool FUSE, bool PAIR>
 cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  using C = GCfg<BN, ACT == 2, FUSE>;
-  auto k = mx4_gemm_kernel<BN, T, ACT, FUSE>;
+  using C = GCfg<BN, ACT == 2, FUSE, PAIR>;
+  constexpr int TM = PAIR ? 2 * kGBM : kGBM;
+  auto k = mx4_gemm_kernel<BN, T, ACT, FUSE, PAIR>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -616,7 +705,7 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
     ready[dev].store(true, std::memory_order_release);
   }
   const int kp = mx_kp(a.K), nout = ACT == 2 ? a.N / 2 : a.N;
-  CUtensorMap mx, mw, my, mr;
+  CUtensorMap mx, mw, my, mr, mxs, mws;
   auto codes = [&](CUtensorMap* m, const uint8_t* base, int rows, uint32_t box_rows) {
     const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)rows}, str[1] = {(uint64_t)kp / 2};
     const uint32_t box[2] = {128, box_rows};
@@ -628,7 +717,7 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
     return make_tmap(m, base, 2, dims, str, box, C::kPW == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                      CU_TENSOR_MAP_DATA_TYPE_UINT16);
   };
-  if (!codes(&mw, a.wcodes, a.N, BN) || !panel(&my, a.y)) return cudaErrorInvalidValue;
+  if (!codes(&mw, a.wcodes, a.N, C::kBRows) || !panel(&my, a.y)) return cudaErrorInvalidValue;
   mr = my;
   if (a.residual && !panel(&mr, a.residual)) return cudaErrorInvalidValue;
   if constexpr (FUSE) {
@@ -639,19 +728,38 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   } else {
     if (!codes(&mx, a.xcodes, a.M, kGBM)) return cudaErrorInvalidValue;
   }
+  mxs = mws = mw;
+  if constexpr (PAIR) {  // scale tiles as rows of 32-bit words, two of 512 bytes at a time
+    auto scales = [&](CUtensorMap* m, const uint8_t* base, int rows) {
+      const uint64_t dims[2] = {(uint64_t)mx_ktiles(a.K) * 128, (uint64_t)mx_rtiles(rows)}, str[1] = {dims[0] * 4};
+      const uint32_t box[2] = {256, 1};
+      return make_tmap(m, base, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_DATA_TYPE_UINT32);
+    };
+    if (!scales(&mxs, a.xscales, a.M) || !scales(&mws, a.wscales, a.N)) return cudaErrorInvalidValue;
+  }
   GemmMx4Dev p;
   p.M = a.M; p.N = a.N; p.K = a.K;
   p.xs = a.xscales; p.ws = a.wscales; p.bias = a.bias; p.residual = a.residual != nullptr; p.err = err;
-  const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + BN - 1) / BN);
-  const int grid = (int)std::min<long long>(tiles, num_sms());
-  return launch_kernel(k, dim3(grid), dim3(C::kThreads), C::kSmem, s, 0, mx, mw, my, mr, p);
+  const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + BN - 1) / BN);
+  if (tiles > (1ll << 30)) return cudaErrorInvalidValue;  // the walk counts tiles in 32 bits
+  const int teams = (int)std::min<long long>(tiles, PAIR ? num_sms() / 2 : num_sms());
+  return launch_kernel(k, dim3(PAIR ? 2 * teams : teams), dim3(C::kThreads), C::kSmem, s, PAIR ? 2 : 0, mx, mw, my, mr, mxs,
+                       mws, p);
 }
+
+// Pairs from this many stages (K > 1792) and two rounds of tiles on. Measured on B200, pairs against single CTAs: 65536 x
+// 640 x 2560 62.4 / 66.6 us, 20000 x 1280 x 5120 63.3 / 68.8 us, but 8192 x 2560 x 1280 23.5 / 20.4 us and 32768 x 640 x
+// 640 23.9 / 17.6 us. (One CTA on 256-wide tiles, as two halves with three accumulators, measured no faster than 128.)
+constexpr int kPairStages = 8;
 
 template <typename T, int ACT>
 cudaError_t gemm_bn(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + 127) / 128);
-  if (a.x) return launch_gemm_mx4<64, T, ACT, true>(a, err, s);
-  return tiles >= num_sms() ? launch_gemm_mx4<128, T, ACT, false>(a, err, s) : launch_gemm_mx4<64, T, ACT, false>(a, err, s);
+  if (a.x) return launch_gemm_mx4<64, T, ACT, true, false>(a, err, s);
+  if (tiles >= 2 * num_sms() && (mx_kp(a.K) + kGStageCols - 1) / kGStageCols >= kPairStages)
+    return launch_gemm_mx4<128, T, ACT, false, true>(a, err, s);
+  return tiles >= num_sms() ? launch_gemm_mx4<128, T, ACT, false, false>(a, err, s)
+                            : launch_gemm_mx4<64, T, ACT, false, false>(a, err, s);
 }
 
 // The fused form while a block quantises at most this many stages (256 columns of 128 rows, about 1.3 us each). Measured

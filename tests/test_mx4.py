@@ -267,7 +267,9 @@ def weight(sdg, N, K, seed):
 SHAPES = [(1, 8, 32), (1, 1280, 1280), (2, 320, 33), (3, 72, 96), (4, 2560, 320), (8, 640, 640), (16, 1280, 320),
           (17, 24, 64), (33, 136, 352), (64, 64, 1000), (65, 1280, 5120), (127, 320, 768), (128, 128, 128),
           (129, 136, 160), (154, 2560, 768), (256, 256, 256), (300, 200, 2560), (512, 1280, 1280), (1000, 960, 320),
-          (2048, 640, 2560), (5000, 320, 320), (8192, 320, 320)]
+          (2048, 640, 2560), (5000, 320, 320), (8192, 320, 320), (20001, 320, 64),
+          # long rows and many tiles: CTA pairs, with half a row tile and a w tile that one CTA has no row of
+          (9985, 520, 2560), (20001, 200, 1800)]
 
 
 @pytest.mark.gpu
@@ -294,7 +296,7 @@ def test_linear(sdg, cuda, M, N, K, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K", [(1, 64, 64), (5, 64, 96), (200, 192, 320)])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 64), (5, 64, 96), (200, 192, 320), (5000, 320, 320), (19999, 320, 1824)])
 def test_linear_output_bounds_and_in_place(sdg, cuda, M, N, K):
     """Nothing is written around y; y may be the residual itself."""
     wc, ws = weight(sdg, N, K, 2)
