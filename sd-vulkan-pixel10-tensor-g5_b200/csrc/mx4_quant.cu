@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
 // Two launches. Statistics: each block reads one chunk of an image's pixels (about 32 KB, all channels) once and
 // writes each group's (mean, M2 = sum of squared differences from that mean) over the chunk. Apply: each block
 // merges the chunks' pairs of the groups its tiles need, in chunk order, then normalises, activates and quantises one to
-// four tiles of the same channels. Threads' and chunks' pairs merge by Chan,
+// eight tiles of the same channels. Threads' and chunks' pairs merge by Chan,
 // Golub and LeVeque's update of (n, mean, M2). Chunks depend on (HW, C) alone: an image's result does
 // not depend on the batch, and no atomics make the order of a sum vary. The second read of x comes from L2 while an
 // input fits it.
@@ -351,23 +351,27 @@ __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x,
   }
 }
 
-// (mean, rstd) of group g from the chunks' pairs at part[k * groups + g]; all lanes of the warp call it.
+// (mean, rstd) of group g from the chunks' pairs at part[k * groups + g]; the eight lanes of a group call it together, a
+// lane taking every eighth chunk. (Pairs kept in registers between the two sums spill: the tile's loads are in flight.)
 __device__ __forceinline__ float2 gn_merge(const float2* part, int g, int groups, int chunks, int chunk, int HW, int cpg,
                                            float eps) {
-  const int lane = threadIdx.x & 31;
+  const int sub = threadIdx.x & 7;
+  auto pixels = [&](int k) { return (float)(min(HW, (k + 1) * chunk) - k * chunk); };
   float s = 0.f;
-  for (int k = lane; k < chunks; k += 32) s += (float)(min(HW, (k + 1) * chunk) - k * chunk) * part[(size_t)k * groups + g].x;
+#pragma unroll 2
+  for (int k = sub; k < chunks; k += 8) s = fmaf(pixels(k), part[(size_t)k * groups + g].x, s);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   const float mu = s / (float)HW;
   float m2 = 0.f;
-  for (int k = lane; k < chunks; k += 32) {
-    const float2 a = part[(size_t)k * groups + g];
-    const float d = a.x - mu;
-    m2 += a.y + (float)(min(HW, (k + 1) * chunk) - k * chunk) * cpg * d * d;
+#pragma unroll 2
+  for (int k = sub; k < chunks; k += 8) {
+    const float2 v = part[(size_t)k * groups + g];
+    const float d = v.x - mu;
+    m2 += fmaf(pixels(k) * cpg * d, d, v.y);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+  for (int o = 4; o; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
   return make_float2(mu, rsqrtf(m2 / ((float)HW * cpg) + eps));
 }
 
@@ -445,11 +449,11 @@ __global__ void __launch_bounds__(kQThreads, 3) mx4_gn_apply_kernel(const T* x, 
       have0 = img0;
       have1 = img1;
       if (p.chunks > 1) {
-        for (int i = threadIdx.x >> 5; i < imgs * ng; i += kQThreads / 32) {
-          const int im = i / ng, g = i - im * ng;
+        for (int i = threadIdx.x >> 3; i < (imgs * ng + 3) / 4 * 4; i += kQThreads / 8) {  // whole warps
+          const int q = min(i, imgs * ng - 1), im = q / ng, g = q - im * ng;
           const float2 st = gn_merge(p.part + (size_t)(img0 + im) * p.chunks * p.groups, g_lo + g, p.groups, p.chunks,
                                      p.chunk, p.HW, cpg, p.eps);
-          if ((threadIdx.x & 31) == 0) table[im * kMxTileCols + g] = st;
+          if ((threadIdx.x & 7) == 0) table[im * kMxTileCols + g] = st;
         }
         __syncthreads();
       }
@@ -577,7 +581,7 @@ cudaError_t groupnorm_t(const Mx4GroupNormArgs& a, cudaStream_t s) {
   const int rts = mx_rtiles(p.M), kts = mx_ktiles(a.C);
   // tiles per block: fewest rounds of blocks (three per SM) weighted by a block's work, a merge counting half a tile
   double best = 1e30;
-  for (int n = 1; n <= 4; ++n) {
+  for (int n = 1; n <= 8; ++n) {
     const long long blocks = (long long)((rts + n - 1) / n) * kts, slots = 3ll * num_sms();
     const double cost = (double)((blocks + slots - 1) / slots) * (n + 0.5);
     if (cost < best) { best = cost; p.tiles = n; }
