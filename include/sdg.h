@@ -302,7 +302,7 @@ SDG_API int sdg_upsample_conv3x3(const uint16_t* x, int B, int H, int W, int Ci,
  *          (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of tile (r / 128, b / 4); bytes of no block are zero.
  * Quantisation of a block: exponent e = max(floor(log2(max|x|)) - 2, -127), codes = x / 2^e rounded to
  * nearest even and saturated at +-6; a block holding an infinity or a NaN gets the exponent NaN (255) and
- * reads back as 32 NaNs. An operand serves as activations (x) or as weights (w, one row per output). */
+ * reads back as 32 NaNs. R up to 2^30, K up to 2^23. An operand serves as activations (x) or as weights (w, one row per output). */
 enum { SDG_F16 = 0, SDG_BF16 = 1, SDG_F32 = 2 }; /* element types of the functions below */
 
 /* Bytes of the two arrays of an [R, K] operand (0 on bad input). */
@@ -320,7 +320,7 @@ SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int 
 
 /* y[M,N] = act(x w^T + bias + residual) for MXFP4 x [M, K] and w [N, K], fp32 accumulation. bias [N] fp32
  * (may be NULL); residual [M, N] and y of type dtype (SDG_F16 or SDG_BF16), 16-byte aligned; y may be the
- * residual itself. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of 16 as for sdg_linear,
+ * residual itself, and overlaps no other argument. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of 16 as for sdg_linear,
  * y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above. */
 SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
                            const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,

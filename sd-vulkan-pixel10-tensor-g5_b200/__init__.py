@@ -501,6 +501,8 @@ def _mx4_device(t) -> int:
 
 
 def _mx4_scale_shape(rows: int, half: int):
+    if rows > 1 << 30 or half > 1 << 22:  # past what the C entries count in 32 bits
+        raise SdgError(3, f"an operand has at most 2^30 rows and 2^23 columns, not {rows} x {2 * half}")
     return ((rows + 127) // 128, (half + 63) // 64, 512)
 
 
@@ -540,10 +542,11 @@ def _mx4_operand(out, rows: int, half: int, like, dev: int, extra: int = 0):
     """The (codes, scales) pair to write into, with both pointers; a pair allocated here has ``extra`` bytes behind it."""
     U8 = _torch.uint8
     if out is None:  # one allocation for both arrays (the scales on a 512-byte boundary behind the codes)
-        rt, kt, n = (rows + 127) // 128, (half + 63) // 64, (rows * half + 511) // 512 * 512
+        rt, kt, _ = shape = _mx4_scale_shape(rows, half)
+        n = (rows * half + 511) // 512 * 512
         both = like.new_empty(n + rt * kt * 512 + extra, dtype=U8)
         p = both.data_ptr()
-        return both.as_strided((rows, half), (half, 1)), both.as_strided((rt, kt, 512), (kt * 512, 512, 1), n), p, p + n
+        return both.as_strided((rows, half), (half, 1)), both.as_strided(shape, (kt * 512, 512, 1), n), p, p + n
     codes, scales = out
     return (codes, scales, _mx4_arg(codes, "codes", dev, U8, (rows, half)),
             _mx4_arg(scales, "scales", dev, U8, _mx4_scale_shape(rows, half)))
@@ -557,7 +560,7 @@ def quantize_mx4(x, out=None, stream=None):
     _mx4_torch()
     dev = _mx4_device(x)
     dt = _mx4_dtype(x.dtype)
-    R, K, ldx = _mx4_rows(x)
+    R, K, ldx = _mx4_rows(x)  # (the size limits are checked with the operand's shape)
     codes, scales, pc, ps = _mx4_operand(out, R, (K + 31) // 32 * 16, x, dev)
     _mx4_call(lib().sdg_quantize_mx4, dev, x.data_ptr(), dt, R, K, ldx, pc, ps)
     return codes, scales
@@ -592,7 +595,8 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
     """y [M, N] = act(x w^T + bias + residual) with both operands in MXFP4 and fp32 accumulation. x is [M, K]
     fp16 / bf16 (quantised on the way; y has its type), or the codes [M, Kp/2] of an operand whose scales are
     ``xscale`` (y has ``dtype``, fp16 by default). w: ``quantize_mx4`` of the [N, K] weight; act 2 = GEGLU on rows
-    packed by ``pack_geglu_weight`` before quantising, y [M, N/2]. ``out`` may be the residual."""
+    packed by ``pack_geglu_weight`` before quantising, y [M, N/2]. ``out`` may be the
+    residual, and overlaps no other argument."""
     if stream is not None:
         return _mx4_on(stream, x, lambda: linear_mx4(x, wcodes, wscales, bias, residual, act, xscale, dtype, out, err_word))
     T = _mx4_torch()
@@ -624,6 +628,7 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
     else:
         py = _mx4_arg(out, "out", dev, dt, shape)
     if xscale is None:
+        _mx4_scale_shape(M, half)
         px, ps, L = x.data_ptr(), None, lib()
         nb = L.sdg_linear_mx4_scratch_bytes(px, M, K, ldx, N)
         if nb:
@@ -651,7 +656,9 @@ def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=
     px = _mx4_arg(x, "x", dev, x.dtype, (B, HW, C))
     pg = _mx4_arg(gamma, "gamma", dev, T.float32, (C,))
     pb = _mx4_arg(beta, "beta", dev, T.float32, (C,))
-    need, half = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups), (C + 31) // 32 * 16
+    half = (C + 31) // 32 * 16
+    _mx4_scale_shape(B * HW, half)
+    need = lib().sdg_groupnorm_mx4_scratch_bytes(B, HW, C, groups)
     codes, scales, pc, ps = _mx4_operand(out, B * HW, half, x, dev, need if stats is None else 0)
     if stats is not None:
         pt = _mx4_arg(stats, "stats", dev, T.float32, stats.shape)
@@ -662,8 +669,7 @@ def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=
     else:
         stats = x.new_empty(need // 4 + 1, dtype=T.float32)
         pt = stats.data_ptr()
-    _mx4_call(lib().sdg_groupnorm_mx4, dev, px, dt, B, HW, C, groups, pg, pb, eps,
-              int(silu), pc, ps, pt)
+    _mx4_call(lib().sdg_groupnorm_mx4, dev, px, dt, B, HW, C, groups, pg, pb, eps, int(silu), pc, ps, pt)
     return codes, scales
 
 

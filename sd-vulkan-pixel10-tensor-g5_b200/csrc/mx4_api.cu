@@ -44,13 +44,14 @@ int status(cudaError_t e, const char* what) {
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 size_t elem_bytes(int dtype) { return dtype == sdg::kF32 ? 4 : 2; }
-// grid.y walks the 128-column scale tiles
-constexpr int kMaxK = 65535 * sdg::kMxTileCols;
+// Rows and columns that 32-bit row, column and tile numbers hold with room for a tile behind the last.
+constexpr int kMaxK = 1 << 23, kMaxRows = 1 << 30;
+bool bad_size(int M, int K) { return M <= 0 || K <= 0 || M > kMaxRows || K > kMaxK; }
 
 int linear_check(const char* what, int M, int K, const uint8_t* wcodes, const uint8_t* wscales, const float* bias, int N,
                  const void* residual, int act, int dtype, const void* y) {
   const std::string w(what);
-  if (!wcodes || !wscales || !y || M <= 0 || K <= 0 || N <= 0 || K > kMaxK || act < 0 || act > 2)
+  if (!wcodes || !wscales || !y || bad_size(M, K) || bad_size(N, K) || act < 0 || act > 2)
     return op_fail(SDG_ERR_ARG, w + ": bad arguments");
   if (dtype != sdg::kF16 && dtype != sdg::kBF16) return op_fail(SDG_ERR_ARG, w + ": dtype must be fp16 or bf16");
   if (act == 2 && residual) return op_fail(SDG_ERR_ARG, w + ": GEGLU takes no residual");
@@ -78,15 +79,15 @@ int linear_run(sdg::Mx4LinearArgs a, int M, int K, const uint8_t* wcodes, const 
 extern "C" {
 
 SDG_API size_t sdg_mx4_code_bytes(int M, int K) {
-  return M <= 0 || K <= 0 || K > kMaxK ? 0 : (size_t)M * (sdg::mx_kp(K) / 2);
+  return bad_size(M, K) ? 0 : (size_t)M * (sdg::mx_kp(K) / 2);
 }
 SDG_API size_t sdg_mx4_scale_bytes(int M, int K) {
-  return M <= 0 || K <= 0 || K > kMaxK ? 0 : (size_t)sdg::mx_rtiles(M) * sdg::mx_ktiles(K) * sdg::kMxTileBytes;
+  return bad_size(M, K) ? 0 : (size_t)sdg::mx_rtiles(M) * sdg::mx_ktiles(K) * sdg::kMxTileBytes;
 }
 
 SDG_API int sdg_quantize_mx4(const void* x, int dtype, int M, int K, int64_t ldx, uint8_t* codes, uint8_t* scales,
                              void* stream) {
-  if (!x || !codes || !scales || M <= 0 || K <= 0 || K > kMaxK || ldx < 0)
+  if (!x || !codes || !scales || bad_size(M, K) || ldx < 0)
     return op_fail(SDG_ERR_ARG, "quantize_mx4: bad arguments");
   if (dtype < sdg::kF16 || dtype > sdg::kF32) return op_fail(SDG_ERR_ARG, "quantize_mx4: dtype must be fp16, bf16 or fp32");
   if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(x, elem_bytes(dtype)))
@@ -97,7 +98,7 @@ SDG_API int sdg_quantize_mx4(const void* x, int dtype, int M, int K, int64_t ldx
 
 SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int M, int K, int dtype, void* y,
                                void* stream) {
-  if (!y || !codes || !scales || M <= 0 || K <= 0 || K > kMaxK)
+  if (!y || !codes || !scales || bad_size(M, K))
     return op_fail(SDG_ERR_ARG, "dequantize_mx4: bad arguments");
   if (dtype < sdg::kF16 || dtype > sdg::kF32)
     return op_fail(SDG_ERR_ARG, "dequantize_mx4: dtype must be fp16, bf16 or fp32");
@@ -146,7 +147,7 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
 }
 
 SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK || sdg::mx4_linear_takes_x(x, M, K, ldx, N)) return 0;
+  if (bad_size(M, K) || N <= 0 || sdg::mx4_linear_takes_x(x, M, K, ldx, N)) return 0;
   return code_space(M, K) + sdg_mx4_scale_bytes(M, K);
 }
 
@@ -161,8 +162,8 @@ SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, in
   if (!x || !gamma || !beta || !codes || !scales || !stats_scratch || B <= 0 || HW <= 0 || C <= 0 || groups <= 0)
     return op_fail(SDG_ERR_ARG, "groupnorm_mx4: bad arguments");
   if (dtype != sdg::kF16 && dtype != sdg::kBF16) return op_fail(SDG_ERR_ARG, "groupnorm_mx4: dtype must be fp16 or bf16");
-  if (C % 8 || C % groups || C > 4096 || B > 65535 || (int64_t)B * HW > INT32_MAX)
-    return op_fail(SDG_ERR_SHAPE, "groupnorm_mx4: C must be a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW below 2^31");
+  if (C % 8 || C % groups || C > 4096 || B > 65535 || (int64_t)B * HW > kMaxRows)
+    return op_fail(SDG_ERR_SHAPE, "groupnorm_mx4: C must be a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW at most 2^30");
   if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(stats_scratch, 8) || !aligned(gamma, 4) ||
       !aligned(beta, 4))
     return op_fail(SDG_ERR_ARG, "groupnorm_mx4: x, codes and scales must be 16-byte aligned");

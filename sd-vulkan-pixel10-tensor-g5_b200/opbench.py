@@ -97,6 +97,26 @@ def build_ops(sdg, dev):
         yl = torch.empty_like(xl)
         ops[f"layernorm_{M}_{C}"] = (lambda xl=xl, gl=gl, bl=bl, yl=yl: sdg.layernorm(xl, gl, bl, out=yl), 0.0,
                                      2.0 * 2 * M * C)
+    for M, C in ((8192, 320), (65536, 2560)):                               # MXFP4 operands: quantise and read back
+        xq = torch.randn(M, C, device=dev).half()
+        qq = sdg.quantize_mx4(xq)
+        ops[f"quantize_mx4_{M}_{C}"] = (lambda xq=xq, qq=qq: sdg.quantize_mx4(xq, out=qq), 0.0, M * C * (2 + 17 / 32))
+        ops[f"dequantize_mx4_{M}_{C}"] = (lambda xq=xq, qq=qq: sdg.dequantize_mx4(*qq, out=xq), 0.0, M * C * (2 + 17 / 32))
+    for M, N, K, act, res in ((8192, 320, 320, 0, True), (8192, 2560, 320, 2, False), (65536, 640, 2560, 0, True)):
+        q4 = sdg.quantize_mx4(torch.randn(M, K, device=dev).half())
+        w4 = sdg.quantize_mx4(0.02 * torch.randn(N, K, device=dev))
+        b4 = torch.zeros(N, device=dev)
+        r4 = torch.randn(M, N, device=dev).half() if res else None
+        y4 = torch.empty((M, N // 2 if act == 2 else N), dtype=torch.float16, device=dev)
+        ops[f"linear_mx4_{M}_{N}_{K}"] = (lambda q4=q4, w4=w4, b4=b4, r4=r4, y4=y4, act=act: sdg.linear_mx4(
+            q4[0], *w4, b4, residual=r4, act=act, xscale=q4[1], out=y4), 2.0 * M * N * K, 0.0)
+    for Bg, C, H in ((B, 320, 64), (B, 1280, 8), (64, 640, 32)):            # GroupNorm + SiLU into an MXFP4 operand
+        x4 = torch.randn(Bg, H * H, C, device=dev).half()
+        g4, t4 = torch.ones(C, device=dev), torch.zeros(C, device=dev)
+        o4 = sdg.groupnorm_mx4(x4, g4, t4, 1e-5, True)
+        s4 = torch.empty(sdg.lib().sdg_groupnorm_mx4_scratch_bytes(Bg, H * H, C, 32) // 4 + 1, device=dev)
+        ops[f"gn_silu_mx4_{Bg}_{C}_{H}"] = (lambda x4=x4, g4=g4, t4=t4, o4=o4, s4=s4: sdg.groupnorm_mx4(
+            x4, g4, t4, 1e-5, True, out=o4, stats=s4), 0.0, Bg * H * H * C * (2 + 17 / 32))
     xt = rn(64)
     yt = torch.empty_like(xt)
     ops["launch_floor_add64"] = (lambda: sdg.add(xt, xt, out=yt), 0.0, 0.0)   # per-launch floor in a graph

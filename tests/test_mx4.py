@@ -77,6 +77,7 @@ def test_sizes(sdg):
     L = sdg.lib()
     assert L.sdg_mx4_code_bytes(3, 33) == 3 * 32 and L.sdg_mx4_scale_bytes(3, 33) == 512
     assert L.sdg_mx4_code_bytes(129, 320) == 129 * 160 and L.sdg_mx4_scale_bytes(129, 320) == 2 * 3 * 512
+    assert L.sdg_mx4_code_bytes((1 << 30) + 1, 5) == 0 and L.sdg_mx4_scale_bytes(5, (1 << 23) + 1) == 0
     assert L.sdg_mx4_code_bytes(0, 5) == 0 and L.sdg_mx4_scale_bytes(5, -1) == 0
     need = L.sdg_linear_mx4_scratch_bytes
     assert need(16, 3, 33, 33, 64) == 0 and need(16, 100, 320, 320, 64) == 0   # few rows, small products: no scratch
@@ -95,7 +96,7 @@ def test_refusals_without_gpu(sdg):
     L = sdg.lib()
     keep, p = _addr()
     q = lambda **k: L.sdg_quantize_mx4(*({"x": p, "dt": 0, "R": 2, "K": 32, "ld": 32, "c": p, "s": p, "st": None} | k).values())
-    assert q(x=None) == q(c=None) == q(s=None) == q(R=0) == q(K=0) == q(ld=-1) == q(dt=3) == q(dt=-1) == SDG_ERR_ARG
+    assert q(x=None) == q(c=None) == q(s=None) == q(R=0) == q(K=0) == q(ld=-1) == q(dt=3) == q(dt=-1) == q(R=(1 << 30) + 1) == SDG_ERR_ARG
     assert q(c=p + 8) == q(s=p + 4) == q(x=p + 1) == SDG_ERR_ARG
     d = lambda **k: L.sdg_dequantize_mx4(*({"c": p, "s": p, "R": 2, "K": 32, "dt": 0, "y": p, "st": None} | k).values())
     assert d(c=None) == d(s=None) == d(y=None) == d(R=0) == d(K=-1) == d(dt=7) == d(y=p + 1) == d(c=p + 2) == SDG_ERR_ARG
@@ -114,7 +115,7 @@ def test_refusals_without_gpu(sdg):
                                            "silu": 0, "c": p, "s": p, "scr": p, "st": None} | k).values())
     assert g(x=None) == g(ga=None) == g(c=None) == g(scr=None) == g(B=0) == g(HW=0) == g(C=0) == g(G=0) == SDG_ERR_ARG
     assert g(dt=2) == g(x=p + 2) == g(c=p + 8) == g(scr=p + 4) == SDG_ERR_ARG
-    assert g(C=60, G=4) == g(C=64, G=7) == g(B=65536) == SDG_ERR_SHAPE
+    assert g(C=60, G=4) == g(C=64, G=7) == g(B=65536) == g(C=4104, G=8) == g(B=2, HW=1 << 30) == SDG_ERR_SHAPE
     assert "groupnorm_mx4" in sdg.last_error()
     del keep
 
@@ -567,3 +568,60 @@ def test_side_streams(sdg, cuda, block):
         streams[0].synchronize()
         assert torch.equal(y, base)
         del junk
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import importlib
+sdg = importlib.import_module({pkg!r})
+x = torch.randn(300, 320, device="cuda").half()
+big = torch.randn(8192, 320, device="cuda").half()
+ga, be = torch.ones(320, device="cuda"), torch.zeros(320, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    w = sdg.quantize_mx4(big[:2560])
+    a = sdg.linear_mx4(x, *w)
+    b = sdg.linear_mx4(big, *w, act=2)
+    q = sdg.groupnorm_mx4(big.view(2, 4096, 320), ga, be, 1e-5, True)
+    c = sdg.linear_mx4(q[0], *w, xscale=q[1])
+    d = sdg.dequantize_mx4(*w)
+g.replay()
+torch.cuda.synchronize()
+w2 = sdg.quantize_mx4(big[:2560])
+q2 = sdg.groupnorm_mx4(big.view(2, 4096, 320), ga, be, 1e-5, True)
+assert torch.equal(w[0], w2[0]) and torch.equal(w[1], w2[1]) and torch.equal(d, sdg.dequantize_mx4(*w2))
+assert torch.equal(a, sdg.linear_mx4(x, *w2)) and torch.equal(b, sdg.linear_mx4(big, *w2, act=2))
+assert torch.equal(c, sdg.linear_mx4(q2[0], *w2, xscale=q2[1]))
+print("captured")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture(cuda):
+    """In a fresh process the first call of every operator may come while a stream is being captured."""
+    import subprocess
+    import sys
+
+    from conftest import PKG, ROOT
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=ROOT, pkg=PKG)], capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_views_of_unaligned_storage(sdg, cuda):
+    """x that starts off a 16-byte boundary, or whose rows do, goes another way to the same result."""
+    K, N = 320, 256
+    wc, ws = weight(sdg, N, K, 3)
+    for M in (1, 5, 64, 300):
+        flat = rnd(M * (K + 8) + 8, seed=M, dtype=torch.float16)
+        want = None
+        for first, ld in ((0, K), (1, K), (8, K + 8), (3, K + 3)):
+            x = flat[first:first + M * ld].view(M, ld)[:, :K]
+            src = rnd(M, K, seed=7, dtype=torch.float16)
+            x.copy_(src)
+            y = sdg.linear_mx4(x, wc, ws)
+            want = y if want is None else want
+            assert torch.equal(y, want)
