@@ -216,11 +216,9 @@ cudaError_t launch_rows(const Mx4LinearArgs& a, cudaStream_t s) {
 // 128 rows x 128 columns of x into a ring by TMA and sixteen more quantise them into the code stages. (Loading x into
 // registers a stage ahead instead ran four times slower: the loads in flight share the scoreboard that the pass in
 // hand waits on.) Every n tile quantises its rows of x again: for small products only.
-// n is the fastest tile index: the tiles in flight share rows of x, and w
-// (at most a few MB) stays in L2.
+// n is the fastest tile index: the tiles in flight share rows of x, and w (at most a few MB) stays in L2.
 constexpr int kGBM = 128;
 constexpr int kGStageCols = 256;  // K columns per stage: one 128-byte swizzled row of codes
-
 constexpr int kGQuantWarps = 16;
 constexpr int kGRawStages = 3;
 constexpr uint32_t kGRawBytes = kGBM * 128 * 2;  // 128 columns of 16 bits, as two 128 B-swizzled boxes of 64
@@ -774,7 +772,9 @@ bool linear_rows(int M, int K) { return M <= 8 && (size_t)8 * (mx_kp(K) / 2 + mx
 template <typename T>
 cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   if (linear_rows(a.M, a.K)) {
-    return a.M == 1 ? launch_rows<T, 1>(a, s) : a.M == 2 ? launch_rows<T, 2>(a, s) : a.M <= 4 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
+    if (a.M == 1) return launch_rows<T, 1>(a, s);
+    if (a.M == 2) return launch_rows<T, 2>(a, s);
+    return a.M <= 4 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
   }
   switch (a.act) {
     case 1: return gemm_bn<T, 1>(a, err, s);

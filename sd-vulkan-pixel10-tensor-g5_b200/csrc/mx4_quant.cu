@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const uint8_t
 constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 8;         // pixels a thread holds at once
 constexpr int kGnShift = 4;         // pixels that give the shift
-constexpr int kGnPixels = 16;       // pixels per thread and chunk, more where an image would need over kGnMaxChunks
+constexpr int kGnPixels = 16;       // least pixels per thread and chunk of an image of several chunks
 constexpr int kGnMaxC = 4096;
 constexpr int kGnMaxChunks = 256;
 
@@ -247,7 +247,9 @@ struct GnPlan {
 };
 __host__ __device__ inline int gn_rows_par(int C) { return C / 8 >= kGnThreads ? 1 : kGnThreads / (C / 8); }
 GnPlan gn_plan(int HW, int C) {
-  const int unit = gn_rows_par(C) * kGnPixels;
+  // twice the pixels where that leaves eight chunks: a chunk's fixed work weighs less (64 x 1024 x 640 58.8 -> 55.8 us, 2 x
+  // 4096 x 320 12.1 -> 12.5 us); smaller images need the blocks (2 x 64 x 1280 7.5 -> 8.8 us)
+  const int par = gn_rows_par(C), unit = par * (HW >= 16 * kGnPixels * par ? 2 * kGnPixels : kGnPixels);
   const int units = (HW + unit - 1) / unit;
   const int per = (units + kGnMaxChunks - 1) / kGnMaxChunks;
   GnPlan p;
@@ -258,7 +260,7 @@ GnPlan gn_plan(int HW, int C) {
 
 // A thread sums d and d^2 of its n pixels of a channel, d = x - k with k the mean of its first m = min(n, 4) pixels.
 // (k - mean)^2 <= M2 / m (Cauchy), so sum d^2 <= M2 (1 + n / m) and M2 = sum d^2 - (sum d)^2 / n loses at most the
-// factor 1 + n / m (5 at 16 pixels) to cancellation, whatever the data.
+// factor 1 + n / m (9 at 32 pixels) to cancellation, whatever the data.
 template <typename T>
 __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
                                                                   int chunk, float2* part) {
