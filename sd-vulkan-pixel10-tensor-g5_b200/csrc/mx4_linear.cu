@@ -4,7 +4,8 @@
 // (value and gate column for GEGLU) for all rows. A lane takes 16 columns at a time (8 bytes of each operand): the
 // codes decode to fp16 exactly, and the eight products a half of each pair adds up stay exact in fp16 (at most 8 * 36 =
 // 288 in steps of 1/4: 1152 steps, fewer than the 2048 an fp16 significand holds). Block scales, and the sums over
-// blocks, are fp32. A plain x is quantised by every block itself, so that the whole call is one launch: it is bound by
+// blocks, are fp32. Of two scales the smaller multiplies a sum first: that product (k / 4 2^e with k <= 2304, e >= -127) is
+// exact, and where it overflows the true one does too, so a finite term stays finite and a zero one zero. A plain x is quantised by every block itself, so that the whole call is one launch: it is bound by
 // launch latency and one pass over the weights.
 #include <algorithm>
 #include <atomic>
@@ -161,7 +162,8 @@ __global__ void __launch_bounds__(kRowsThreads) mx4_rows_kernel(Mx4LinearArgs a)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s = __hfma2(h1[j], wv[w][4 + j], s);
           const float2 f = __half22float2(s);
-          acc[w][m] += (f.x + f.y) * xsc * wsc[w];
+          const uint32_t a = __float_as_uint(xsc), b = __float_as_uint(wsc[w]);  // as integers: a NaN is the larger
+          acc[w][m] += (f.x + f.y) * __uint_as_float(min(a, b)) * __uint_as_float(max(a, b));
         }
       }
     }
