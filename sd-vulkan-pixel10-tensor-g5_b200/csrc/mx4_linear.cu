@@ -247,7 +247,7 @@ struct GCfg {
   static constexpr uint32_t kTmemCols = 2 * BN + 2 * kSfCols <= 256 ? 256 : 512;
   static_assert(2 * BN + 2 * kSfCols <= 512 && kStages >= 3, "tile does not fit");
   static_assert(!FUSE || kGBM == 2 * 4 * kGQuantWarps, "two passes of four rows a warp");
-  static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 4 <= 512, "barriers do not fit");
+  static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 8 <= 512, "barriers do not fit");
 };
 
 // A block's walk over the tiles first, first + step, ... (n fastest), without a division per tile.
@@ -267,6 +267,48 @@ struct TileWalk {
     if (n >= num_n) {
       n -= num_n;
       ++m;
+    }
+  }
+};
+
+// The bounded waits of a block. A wait that expires records its code in the error word and stops the other waits of its block
+// (of both blocks of a pair) through a flag in their shared memory. They do not look at the error word itself: it may be
+// shared with other launches, and one that failed must not end the waits of those that follow.
+template <bool PAIR>
+struct Waits {
+  uint32_t stop;  // shared-memory address of the flag
+  int* err;
+
+  __device__ __forceinline__ bool stopped() const {
+    uint32_t v;
+    asm volatile("ld.volatile.shared::cta.b32 %0, [%1];" : "=r"(v) : "r"(stop) : "memory");
+    return v != 0;
+  }
+  __device__ __forceinline__ void expire(int code) const {
+    atomicCAS(err, 0, code);
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_shared(stop, r)), "r"(1u) : "memory");
+    } else {
+      asm volatile("st.volatile.shared::cta.b32 [%0], %1;" ::"r"(stop), "r"(1u) : "memory");
+    }
+  }
+  // CLUSTER: the peer's arrivals count too
+  template <bool CLUSTER = false>
+  __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code) const {
+    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+    if (done()) return true;
+    const uint64_t t0 = globaltimer();
+    for (uint32_t i = 1;; ++i) {
+      if (done()) return true;
+      if ((i & 255u) == 0u) {
+        if (stopped()) return false;
+        if (globaltimer() - t0 > kWaitTimeoutNs) {
+          expire(code);
+          return false;
+        }
+      }
     }
   }
 };
@@ -298,6 +340,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
   float* sBias = reinterpret_cast<float*>(sSf + S * C::kSfBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sBias + C::kEpiWarps * 64);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + C::kEpiWarps + 2 * kGRawStages);
+  const Waits<PAIR> waits{smem_u32(tmem_slot + 1), p.err};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -316,6 +359,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
   const int nst = (kp + kGStageCols - 1) / kGStageCols;  // stages per tile
 
   if (threadIdx.x == 0) {
+    tmem_slot[1] = 0;  // the waits' stop flag
     for (int s = 0; s < S; ++s) {
       mbar_init(full_bar(s), FUSE ? 1 + kGQuantWarps : 1);
       mbar_init(empty_bar(s), 1);
@@ -379,7 +423,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
       for (int k = 0; k < nst; ++k, ++it) {
         const int s = it % S;
-        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, waits.wait(empty_bar(s), ((it / S) & 1u) ^ 1u, kDevTimeoutEmpty));
         if (!ok) break;
         const uint32_t sfb = (uint32_t)min(2, kts - 2 * k) * kMxTileBytes;  // scale bytes per 128 rows
         const uint32_t dA = smem_u32(smem + s * C::kABytes);
@@ -438,15 +482,14 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
         const int n0 = tw.n * BN;
         const uint32_t acc = tl & 1u;
         const uint32_t free_ph = ((tl >> 1) & 1u) ^ 1u;
-        ok = __all_sync(0xffffffffu, PAIR ? mbar_wait_cluster(tempty_bar(acc), free_ph, p.err, kDevTimeoutAcc)
-                                          : mbar_wait(tempty_bar(acc), free_ph, p.err, kDevTimeoutAcc));
+        ok = __all_sync(0xffffffffu, waits.template wait<PAIR>(tempty_bar(acc), free_ph, kDevTimeoutAcc));
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         const uint32_t n_off = (uint32_t)(n0 % kMxTileRows) / 32u;  // BN = 64: the tile's half of its scale tile
         for (int k = 0; k < nst; ++k, ++it) {
           const int s = it % S;
-          ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (it / S) & 1u, p.err, kDevTimeoutFull));
+          ok = __all_sync(0xffffffffu, waits.wait(full_bar(s), (it / S) & 1u, kDevTimeoutFull));
           if (!ok) break;
           const uint32_t sf = tmem_base + 2 * BN + (it & 1u) * C::kSfCols;
           const uint32_t dS = smem_u32(sSf + s * C::kSfBytes);
@@ -496,7 +539,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       const int m0 = tw.m * kGBM;
       for (int k = 0; k < nraw; ++k, ++it) {
         const int s = it % kGRawStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, waits.wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, kDevTimeoutEmpty));
         if (!ok) break;
         const uint32_t d = smem_u32(sRaw + s * kGRawBytes);
         if (elect_one()) {
@@ -518,14 +561,14 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
     for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
       for (int k = 0; k < nst && ok; ++k, ++it) {
         const int s = it % S;
-        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ((it / S) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, waits.wait(empty_bar(s), ((it / S) & 1u) ^ 1u, kDevTimeoutEmpty));
         if (!ok) break;
         uint8_t* dA = smem + s * C::kABytes;
         uint8_t* dS = sSf + s * C::kSfBytes;
         const int halves = kp - k * kGStageCols > 128 ? 2 : 1;
         for (int h = 0; h < halves; ++h, ++rit) {
           const int rs = rit % kGRawStages;
-          ok = __all_sync(0xffffffffu, mbar_wait(rfull_bar(rs), (rit / kGRawStages) & 1u, p.err, kDevTimeoutFull));
+          ok = __all_sync(0xffffffffu, waits.wait(rfull_bar(rs), (rit / kGRawStages) & 1u, kDevTimeoutFull));
           if (!ok) break;
           // 64-column box l / 4; its 16-byte chunks are XORed with the row as TMA wrote them
           const uint8_t* src = sRaw + rs * kGRawBytes + (l >> 2) * (kGRawBytes / 2);
@@ -590,9 +633,9 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       if (!p.residual && lane == 0) bulk_wait_read<0>();  // the panel's previous store has read it
       __syncwarp();
       const uint32_t tl = q * C::kSets + set, acc = tl & 1u;  // the block's tile number, and its accumulator
-      bool ok = mbar_wait(tfull_bar(acc), (tl >> 1) & 1u, p.err, kDevTimeoutAcc);
+      bool ok = waits.wait(tfull_bar(acc), (tl >> 1) & 1u, kDevTimeoutAcc);
       if (ok && p.residual) {
-        ok = mbar_wait(res_bar(w), q & 1u, p.err, kDevTimeoutEmpty);
+        ok = waits.wait(res_bar(w), q & 1u, kDevTimeoutEmpty);
         if (ok) loading = false;
       }
       if (!__all_sync(0xffffffffu, ok)) break;
