@@ -335,6 +335,17 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
                              size_t scratch_bytes, int* err_word, void* stream);
 SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N);
 
+/* Failure-path test: as sdg_selftest_stalled_gemm, for y[M,N] = x w^T + residual (fp16, residual may be NULL). x is an operand's
+ * codes with `xscales`, or with xscales NULL a plain [M, K] that the product quantises itself. `form` names the kernel that the
+ * sizes have to lead to: 1 x quantised on the way, 2 64-wide tiles, 3 128-wide tiles, 4 CTA pairs. In every CTA one
+ * loader stops before its load number `stall_iter`: stall_who 0 the producer (of a pair the even CTA's), 1 the odd CTA's
+ * producer (form 4) or the loader of x (form 1). The call synchronises `stream`, clears the word and returns SDG_ERR_DEVICE
+ * naming the code (SDG_OK would mean that nothing expired). */
+SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
+                                            const uint8_t* wscales, int N, const void* residual, void* y, int form,
+                                            int stall_who, int stall_iter, int wait_limit_us, int* err_word,
+                                            void* stream);
+
 /* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
  * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to
  * 16 bits in between. C a multiple of 8 and of groups, at most 4096. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes

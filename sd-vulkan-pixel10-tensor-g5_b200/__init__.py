@@ -103,6 +103,7 @@ _SIGS = {
     "sdg_dequantize_mx4": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "sdg_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P]),
     "sdg_linear_mx4_x": (_I, [_P, _I, _I, ctypes.c_int64, _P, _P, _P, _I, _P, _I, _I, _P, _P, ctypes.c_size_t, _P, _P]),
+    "sdg_selftest_stalled_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
     "sdg_linear_mx4_scratch_bytes": (ctypes.c_size_t, [_P, _I, _I, ctypes.c_int64, _I]),
     "sdg_groupnorm_mx4": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
     "sdg_groupnorm_mx4_scratch_bytes": (ctypes.c_size_t, [_I, _I, _I, _I]),

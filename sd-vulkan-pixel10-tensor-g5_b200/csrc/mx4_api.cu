@@ -1,5 +1,6 @@
 // mx4_api.cu — C entry points of the MXFP4 operators (include/sdg.h): quantise, read back, linear, GroupNorm
 // into an MXFP4 operand.
+#include <cstdio>
 #include <mutex>
 #include <string>
 
@@ -60,6 +61,22 @@ int linear_check(const char* what, int M, int K, const uint8_t* wcodes, const ui
   if (!aligned(wcodes, 16) || !aligned(wscales, 16) || !aligned(y, 16) || !aligned(residual, 16) || !aligned(bias, 4))
     return op_fail(SDG_ERR_ARG, w + ": weight, scale, residual and output pointers must be 16-byte aligned");
   return SDG_OK;
+}
+
+// Waits for the stream, then reads and clears an error word: SDG_ERR_DEVICE with its code, if it held one.
+int take_code(int* word, cudaStream_t s, const char* what) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyAsync(&v, word, sizeof v, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && v != 0) {
+    e = cudaMemsetAsync(word, 0, sizeof v, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  if (e != cudaSuccess) return status(e, what);
+  if (v == 0) return SDG_OK;
+  char buf[128];
+  snprintf(buf, sizeof buf, "%s: device error word 0x%x (a kernel's bounded wait expired)", what, v);
+  return op_fail(SDG_ERR_DEVICE, buf);
 }
 
 // The codes' part of the scratch, rounded up so that the scales behind it are aligned.
@@ -144,6 +161,37 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
     a.xscales = xs;
   }
   return linear_run(a, M, K, wcodes, wscales, bias, N, residual, act, dtype, y, err_word, s);
+}
+
+SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
+                                            const uint8_t* wscales, int N, const void* residual, void* y, int form,
+                                            int stall_who, int stall_iter, int wait_limit_us, int* err_word,
+                                            void* stream) {
+  const char* what = "selftest_stalled_linear_mx4";
+  int st = linear_check(what, M, K, wcodes, wscales, nullptr, N, residual, 0, sdg::kF16, y);
+  if (st) return st;
+  if (!x || !aligned(x, 16) || !aligned(xscales, 16) || !err_word || stall_iter < 0 || stall_who < 0 || stall_who > 1 ||
+      wait_limit_us <= 0 || wait_limit_us > 2000000)
+    return op_fail(SDG_ERR_ARG, std::string(what) + ": bad arguments");
+  sdg::Mx4LinearArgs a;
+  if (xscales) {
+    a.xcodes = static_cast<const uint8_t*>(x);
+    a.xscales = xscales;
+  } else {
+    if (!sdg::mx4_linear_takes_x(x, M, K, K, N)) return op_fail(SDG_ERR_ARG, std::string(what) + ": not a fused product");
+    a.x = x;
+    a.ldx = K;
+  }
+  a.M = M; a.N = N; a.K = K; a.wcodes = wcodes; a.wscales = wscales; a.residual = residual; a.y = y;
+  const sdg::Mx4Form f = sdg::mx4_linear_form(a);
+  if (f == sdg::kMx4Rows || (int)f != form || (stall_who && f != sdg::kMx4Fused && f != sdg::kMx4Pair))
+    return op_fail(SDG_ERR_ARG, std::string(what) + ": the product does not run in that form");
+  a.test_stall_iter = stall_iter;
+  a.test_stall_who = stall_who;
+  a.wait_limit_ns = 1000ull * (unsigned long long)wait_limit_us;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  st = status(sdg::launch_mx4_linear(a, err_word, s), what);
+  return st ? st : take_code(err_word, s, what);
 }
 
 SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N) {

@@ -247,7 +247,7 @@ struct GCfg {
   static constexpr uint32_t kTmemCols = 2 * BN + 2 * kSfCols <= 256 ? 256 : 512;
   static_assert(2 * BN + 2 * kSfCols <= 512 && kStages >= 3, "tile does not fit");
   static_assert(!FUSE || kGBM == 2 * 4 * kGQuantWarps, "two passes of four rows a warp");
-  static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 8 <= 512, "barriers do not fit");
+  static_assert((2 * kStages + 5 + kEpiWarps + 2 * kGRawStages) * 8 + 12 <= 512, "barriers do not fit");
 };
 
 // A block's walk over the tiles first, first + step, ... (n fastest), without a division per tile.
@@ -278,6 +278,7 @@ template <bool PAIR>
 struct Waits {
   uint32_t stop;  // shared-memory address of the flag
   int* err;
+  unsigned long long limit_ns;
 
   __device__ __forceinline__ bool stopped() const {
     uint32_t v;
@@ -304,7 +305,7 @@ struct Waits {
       if (done()) return true;
       if ((i & 255u) == 0u) {
         if (stopped()) return false;
-        if (globaltimer() - t0 > kWaitTimeoutNs) {
+        if (globaltimer() - t0 > limit_ns) {
           expire(code);
           return false;
         }
@@ -320,6 +321,8 @@ struct GemmMx4Dev {
   const float* bias;
   int residual;
   int* err;
+  unsigned long long wait_ns;  // limit of every bounded wait
+  int stall_it, stall_who;     // failure-path test: loader stall_who stops before its load number stall_it (-1: never)
 };
 
 template <int BN, typename T, int ACT, bool FUSE, bool PAIR>
@@ -340,7 +343,8 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
   float* sBias = reinterpret_cast<float*>(sSf + S * C::kSfBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sBias + C::kEpiWarps * 64);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5 + C::kEpiWarps + 2 * kGRawStages);
-  const Waits<PAIR> waits{smem_u32(tmem_slot + 1), p.err};
+  uint32_t* issued = tmem_slot + 2;  // stages that this CTA's producer has loaded
+  const Waits<PAIR> waits{smem_u32(tmem_slot + 1), p.err, p.wait_ns};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -403,11 +407,13 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
   // unevenly when it ends. Measured on B200, quantise + product in a row: 65536 x 640 x 2560 181 us with a trigger here,
   // 163 us with one after the last MMA, 161 us without; 8192 x 320 x 320 9.3 / 8.3 / 7.8 us.
 
+  uint32_t count = 0;  // stages loaded or filled, raw tiles loaded: what an abort has to wait for
   if (warp == 0) {
     // all lanes walk the loop and wait; one of them issues
     pdl_wait();
     uint32_t it = 0;
     bool ok = true;
+    const int stall_it = p.stall_who == rank ? p.stall_it : -1;
     for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
       const int m0 = tw.m * TM + rank * kGBM, n0 = tw.n * BN;
       const uint8_t* xs = FUSE ? nullptr : p.xs + (size_t)(m0 / kMxTileRows) * kts * kMxTileBytes;
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
       for (int k = 0; k < nst; ++k, ++it) {
         const int s = it % S;
-        ok = __all_sync(0xffffffffu, waits.wait(empty_bar(s), ((it / S) & 1u) ^ 1u, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, waits.wait(empty_bar(s), ((it / S) & 1u) ^ 1u, kDevTimeoutEmpty)) && (int)it != stall_it;
         if (!ok) break;
         const uint32_t sfb = (uint32_t)min(2, kts - 2 * k) * kMxTileBytes;  // scale bytes per 128 rows
         const uint32_t dA = smem_u32(smem + s * C::kABytes);
@@ -455,15 +461,8 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
         __syncwarp();
       }
     }
-    // abort: every copy in flight lands before the shared memory is released
-    if (!ok && lane == 0) {
-      if (rank == 0) {
-        for (uint32_t q = it > (uint32_t)S ? it - S : 0; q < it; ++q)
-          mbar_drain(full_bar(q % S), (q / S) & 1u, p.err, kDevTimeoutDrain);
-      } else {
-        spin_ns(200000);  // the odd CTA cannot see the even CTA's barriers
-      }
-    }
+    count = it;
+    if (lane == 0) *issued = it;
   } else if (warp == 1) {
     if (rank == 0) {
       // all lanes walk the loop and wait; one of them issues
@@ -527,7 +526,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       }
       // every issued copy and MMA has retired before TMEM is released
       __syncwarp();
-      if (lane == 0) mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain);
+      if (lane == 0) mbar_drain(drain_bar, 0, p.err, kDevTimeoutDrain, p.wait_ns);
     }
   } else if (FUSE && warp == 2 + C::kEpiWarps + kGQuantWarps) {
     // x into the raw ring
@@ -535,11 +534,13 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
     const int nraw = (kp + 127) / 128;
     uint32_t it = 0;
     bool ok = true;
+    const int stall_it = p.stall_who == 1 ? p.stall_it : -1;
     for (TileWalk tw(team, teams, num_m, num_n); tw.valid() && ok; tw.next()) {
       const int m0 = tw.m * kGBM;
       for (int k = 0; k < nraw; ++k, ++it) {
         const int s = it % kGRawStages;
-        ok = __all_sync(0xffffffffu, waits.wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, waits.wait(rempty_bar(s), ((it / kGRawStages) & 1u) ^ 1u, kDevTimeoutEmpty)) &&
+             (int)it != stall_it;
         if (!ok) break;
         const uint32_t d = smem_u32(sRaw + s * kGRawBytes);
         if (elect_one()) {
@@ -550,9 +551,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
         __syncwarp();
       }
     }
-    if (!ok && lane == 0)
-      for (uint32_t q = it > (uint32_t)kGRawStages ? it - kGRawStages : 0; q < it; ++q)
-        mbar_drain(rfull_bar(q % kGRawStages), (q / kGRawStages) & 1u, p.err, kDevTimeoutDrain);
+    count = it;
   } else if (FUSE && warp >= 2 + C::kEpiWarps) {
     // quantiser: four rows a pass and warp (64 a pass in all), eight lanes a row, 16 columns a lane
     const int l = lane & 7, r0 = (warp - 2 - C::kEpiWarps) * 4 + (lane >> 3);
@@ -609,6 +608,7 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
         if (lane == 0) mbar_arrive(full_bar(s));
       }
     }
+    count = it;
   } else {
     pdl_wait();
     // set: which tiles (and accumulator); lg: the TMEM lane quadrant a warp may read; pn: its 64 columns
@@ -625,7 +625,8 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       load_res(tw.m, tw.n);
       loading = true;
     }
-    for (uint32_t q = 0; tw.valid(); ++q) {
+    uint32_t q = 0;
+    for (; tw.valid(); ++q) {
       const int m0 = tw.m * TM + rank * kGBM, n = tw.n * BN + pn * 64;
       tw.next();  // from here on the next tile
       bias_s[lane] = p.bias && n + lane < p.N ? p.bias[n + lane] : 0.f;
@@ -713,16 +714,39 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
     }
     if (lane == 0) {
       // abort: a residual copy in flight lands before the shared memory is released
-      if (loading) spin_ns(200000);
+      if (loading) mbar_drain(res_bar(w), q & 1u, p.err, kDevTimeoutDrain, p.wait_ns);
       bulk_wait_read<0>();
     }
   }
   tc_fence_before();
   __syncwarp();
-  if constexpr (PAIR)
-    cluster_sync_all();  // neither CTA frees TMEM or shared memory that the pair still uses
-  else
-    __syncthreads();
+  auto sync_all = [] {
+    if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  };
+  sync_all();  // neither CTA frees TMEM or shared memory that the pair still uses
+  if (waits.stopped()) {
+    // A wait expired (all threads, a pair's too, see the same flag: no wait is left). Every copy in flight lands before the
+    // shared memory is released: each stage's barrier is brought to the end of its phase and waited for. Producers, quantisers
+    // and the two CTAs of a pair are at most S stages apart, so a stage that one side lacks is in its barrier's current phase.
+    if (FUSE && warp >= 2 + C::kEpiWarps && warp < 2 + C::kEpiWarps + kGQuantWarps && lane == 0)
+      for (uint32_t i = count; i < *issued; ++i) mbar_arrive(full_bar(i % S));  // stages loaded, not filled
+    if (FUSE && warp == 2 + C::kEpiWarps + kGQuantWarps && lane == 0)
+      for (uint32_t i = count > (uint32_t)kGRawStages ? count - kGRawStages : 0; i < count; ++i)
+        mbar_drain(rfull_bar(i % kGRawStages), (i / kGRawStages) & 1u, p.err, kDevTimeoutDrain, p.wait_ns);
+    if (warp == 0 && lane == 0 && rank == 0) {
+      uint32_t top = count;
+      if constexpr (PAIR) {
+        const uint32_t odd = ld_cluster(mapa_shared(smem_u32(issued), 1));
+        for (uint32_t i = odd; i < count; ++i) mbar_complete_tx(full_bar(i % S), C::kStageBytes);  // never loaded there
+        for (uint32_t i = count; i < odd; ++i) mbar_arrive_expect_tx(full_bar(i % S), C::kStageBytes);  // never loaded here
+        top = max(count, odd);
+      }
+      for (uint32_t i = top > (uint32_t)S ? top - S : 0; i < top; ++i)
+        mbar_drain(full_bar(i % S), (i / S) & 1u, p.err, kDevTimeoutDrain, p.wait_ns);
+    }
+    __syncwarp();
+    sync_all();
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (PAIR)
@@ -783,6 +807,8 @@ cudaError_t launch_gemm_mx4(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
   GemmMx4Dev p;
   p.M = a.M; p.N = a.N; p.K = a.K;
   p.xs = a.xscales; p.ws = a.wscales; p.bias = a.bias; p.residual = a.residual != nullptr; p.err = err;
+  p.wait_ns = a.wait_limit_ns ? a.wait_limit_ns : kWaitTimeoutNs;
+  p.stall_it = a.test_stall_iter; p.stall_who = a.test_stall_who;
   const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + BN - 1) / BN);
   if (tiles > (1ll << 30)) return cudaErrorInvalidValue;  // the walk counts tiles in 32 bits
   const int teams = (int)std::min<long long>(tiles, PAIR ? num_sms() / 2 : num_sms());
@@ -797,12 +823,12 @@ constexpr int kPairStages = 8;
 
 template <typename T, int ACT>
 cudaError_t gemm_bn(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + 127) / 128);
-  if (a.x) return launch_gemm_mx4<64, T, ACT, true, false>(a, err, s);
-  if (tiles >= 2 * num_sms() && (mx_kp(a.K) + kGStageCols - 1) / kGStageCols >= kPairStages)
-    return launch_gemm_mx4<128, T, ACT, false, true>(a, err, s);
-  return tiles >= num_sms() ? launch_gemm_mx4<128, T, ACT, false, false>(a, err, s)
-                            : launch_gemm_mx4<64, T, ACT, false, false>(a, err, s);
+  switch (mx4_linear_form(a)) {
+    case kMx4Fused: return launch_gemm_mx4<64, T, ACT, true, false>(a, err, s);
+    case kMx4Pair: return launch_gemm_mx4<128, T, ACT, false, true>(a, err, s);
+    case kMx4Wide: return launch_gemm_mx4<128, T, ACT, false, false>(a, err, s);
+    default: return launch_gemm_mx4<64, T, ACT, false, false>(a, err, s);
+  }
 }
 
 // The fused form while a block quantises at most this many stages (256 columns of 128 rows, about 1.3 us each). Measured
@@ -816,7 +842,7 @@ bool linear_rows(int M, int K) { return M <= 8 && (size_t)8 * (mx_kp(K) / 2 + mx
 
 template <typename T>
 cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
-  if (linear_rows(a.M, a.K)) {
+  if (mx4_linear_form(a) == kMx4Rows) {
     if (a.M == 1) return launch_rows<T, 1>(a, s);
     if (a.M == 2) return launch_rows<T, 2>(a, s);
     return a.M <= 4 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
@@ -829,6 +855,14 @@ cudaError_t linear_t(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 }
 
 }  // namespace
+
+Mx4Form mx4_linear_form(const Mx4LinearArgs& a) {
+  if (linear_rows(a.M, a.K)) return kMx4Rows;
+  if (a.x) return kMx4Fused;
+  const long long tiles = (long long)((a.M + kGBM - 1) / kGBM) * ((a.N + 127) / 128);
+  if (tiles >= 2 * num_sms() && (mx_kp(a.K) + kGStageCols - 1) / kGStageCols >= kPairStages) return kMx4Pair;
+  return tiles >= num_sms() ? kMx4Wide : kMx4Narrow;
+}
 
 bool mx4_linear_takes_x(const void* x, int M, int K, long long ldx, int N) {
   if (linear_rows(M, K)) return true;

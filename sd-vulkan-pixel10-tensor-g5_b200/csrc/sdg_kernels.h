@@ -145,7 +145,15 @@ struct Mx4LinearArgs {
   const float* bias = nullptr; const void* residual = nullptr;
   int act = 0, dtype = kF16;
   void* y = nullptr;
+  // Failure-path test only: one loader of each CTA stops before its load number test_stall_iter (-1: never). test_stall_who:
+  // 0 the producer (the even CTA's of a pair), 1 the odd CTA's, or in the fused form the loader of x.
+  int test_stall_iter = -1, test_stall_who = 0;
+  unsigned long long wait_limit_ns = 0;  // limit of every bounded wait (0: kWaitTimeoutNs)
 };
+// The kernel that a product runs on: CUDA cores (few rows); tensor cores with x quantised on the way, 64- or 128-wide tiles,
+// or CTA pairs.
+enum Mx4Form { kMx4Rows = 0, kMx4Fused = 1, kMx4Narrow = 2, kMx4Wide = 3, kMx4Pair = 4 };
+Mx4Form mx4_linear_form(const Mx4LinearArgs& a);
 // Whether the product quantises a plain x itself (few rows, small products); otherwise it wants the operand.
 bool mx4_linear_takes_x(const void* x, int M, int K, long long ldx, int N);
 cudaError_t launch_mx4_linear(const Mx4LinearArgs& a, int* dev_err, cudaStream_t s);
