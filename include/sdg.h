@@ -321,7 +321,8 @@ SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int 
 /* y[M,N] = act(x w^T + bias + residual) for MXFP4 x [M, K] and w [N, K], fp32 accumulation. bias [N] fp32
  * (may be NULL); residual [M, N] and y of type dtype (SDG_F16 or SDG_BF16), 16-byte aligned; y may be the
  * residual itself, and overlaps no other argument. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of 16 as for sdg_linear,
- * y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above. */
+ * y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above; without one, sdg_mx4_status tells
+ * whether the product completed. */
 SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
                            const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,
                            void* y, int* err_word, void* stream);
@@ -335,12 +336,17 @@ SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uin
                              size_t scratch_bytes, int* err_word, void* stream);
 SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N);
 
+/* Waits for `stream`, then returns SDG_ERR_DEVICE if, since the last such call, a product without an err_word of its own left
+ * parts of its y unwritten because a bounded wait expired, on any stream of the current device; SDG_OK otherwise. Not on a
+ * stream that is being captured (SDG_ERR_ARG). */
+SDG_API int sdg_mx4_status(void* stream);
+
 /* Failure-path test: as sdg_selftest_stalled_gemm, for y[M,N] = x w^T + residual (fp16, residual may be NULL). x is an operand's
  * codes with `xscales`, or with xscales NULL a plain [M, K] that the product quantises itself. `form` names the kernel that the
  * sizes have to lead to: 1 x quantised on the way, 2 64-wide tiles, 3 128-wide tiles, 4 CTA pairs. In every CTA one
  * loader stops before its load number `stall_iter`: stall_who 0 the producer (of a pair the even CTA's), 1 the odd CTA's
  * producer (form 4) or the loader of x (form 1). The call synchronises `stream`, clears the word and returns SDG_ERR_DEVICE
- * naming the code (SDG_OK would mean that nothing expired). */
+ * naming the code (SDG_OK would mean that nothing expired). With err_word NULL it only launches: sdg_mx4_status reports. */
 SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
                                             const uint8_t* wscales, int N, const void* residual, void* y, int form,
                                             int stall_who, int stall_iter, int wait_limit_us, int* err_word,

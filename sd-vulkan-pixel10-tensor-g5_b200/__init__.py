@@ -103,6 +103,7 @@ _SIGS = {
     "sdg_dequantize_mx4": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "sdg_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P]),
     "sdg_linear_mx4_x": (_I, [_P, _I, _I, ctypes.c_int64, _P, _P, _P, _I, _P, _I, _I, _P, _P, ctypes.c_size_t, _P, _P]),
+    "sdg_mx4_status": (_I, [_P]),
     "sdg_selftest_stalled_linear_mx4": (_I, [_P, _P, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
     "sdg_linear_mx4_scratch_bytes": (ctypes.c_size_t, [_P, _I, _I, ctypes.c_int64, _I]),
     "sdg_groupnorm_mx4": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
@@ -597,7 +598,8 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
     fp16 / bf16 (quantised on the way; y has its type), or the codes [M, Kp/2] of an operand whose scales are
     ``xscale`` (y has ``dtype``, fp16 by default). w: ``quantize_mx4`` of the [N, K] weight; act 2 = GEGLU on rows
     packed by ``pack_geglu_weight`` before quantising, y [M, N/2]. ``out`` may be the
-    residual, and overlaps no other argument."""
+    residual, and overlaps no other argument. ``err_word``: int32 that the kernel's bounded waits report to; without one
+    ``mx4_status`` tells whether the product completed."""
     if stream is not None:
         return _mx4_on(stream, x, lambda: linear_mx4(x, wcodes, wscales, bias, residual, act, xscale, dtype, out, err_word))
     T = _mx4_torch()
@@ -641,6 +643,14 @@ def linear_mx4(x, wcodes, wscales, bias=None, residual=None, act: int = 0, xscal
         pxs = _mx4_arg(xscale, "xscale", dev, U8, _mx4_scale_shape(M, half))
         _mx4_call(lib().sdg_linear_mx4, dev, px, pxs, M, K, pw, pws, pb, N, pr, act, code, py, pe)
     return out
+
+
+def mx4_status(device=None, stream=None) -> None:
+    """Waits for the current stream of ``device`` (the current one), or for ``stream`` (a raw handle), and raises if, since
+    the last call, a ``linear_mx4`` without an ``err_word`` of its own could not complete on that device."""
+    T = _mx4_torch()
+    with T.cuda.device(device):
+        check(lib().sdg_mx4_status(T.cuda.current_stream().cuda_stream if stream is None else stream))
 
 
 def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=None, stats=None, stream=None):

@@ -17,7 +17,7 @@ namespace {
 using sdg::op_fail;
 
 // The word the kernels' bounded waits report to when the caller passes none: zero-initialised device memory of the
-// library, looked up once per device. The look-up may load the module, so it runs with this thread's
+// library, looked up once per device; sdg_mx4_status reads and clears it. The look-up may load the module, so it runs with this thread's
 // stream-capture mode relaxed: a first call inside a capture is fine.
 static __device__ int g_mx4_err[64];
 std::mutex g_mu;
@@ -170,7 +170,7 @@ SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscale
   const char* what = "selftest_stalled_linear_mx4";
   int st = linear_check(what, M, K, wcodes, wscales, nullptr, N, residual, 0, sdg::kF16, y);
   if (st) return st;
-  if (!x || !aligned(x, 16) || !aligned(xscales, 16) || !err_word || stall_iter < 0 || stall_who < 0 || stall_who > 1 ||
+  if (!x || !aligned(x, 16) || !aligned(xscales, 16) || stall_iter < 0 || stall_who < 0 || stall_who > 1 ||
       wait_limit_us <= 0 || wait_limit_us > 2000000)
     return op_fail(SDG_ERR_ARG, std::string(what) + ": bad arguments");
   sdg::Mx4LinearArgs a;
@@ -190,8 +190,23 @@ SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscale
   a.test_stall_who = stall_who;
   a.wait_limit_ns = 1000ull * (unsigned long long)wait_limit_us;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = status(sdg::launch_mx4_linear(a, err_word, s), what);
-  return st ? st : take_code(err_word, s, what);
+  int* err = err_word ? err_word : default_err_word();
+  if (!err) return op_fail(SDG_ERR_CUDA, std::string(what) + ": no device error word");
+  st = status(sdg::launch_mx4_linear(a, err, s), what);
+  return st || !err_word ? st : take_code(err_word, s, what);
+}
+
+SDG_API int sdg_mx4_status(void* stream) {
+  const char* what = "mx4_status";
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(s, &cap);
+  if (e == cudaErrorStreamCaptureImplicit || (e == cudaSuccess && cap != cudaStreamCaptureStatusNone))
+    return op_fail(SDG_ERR_ARG, std::string(what) + ": the stream is being captured");
+  if (e != cudaSuccess) return status(e, what);
+  int* word = default_err_word();
+  if (!word) return op_fail(SDG_ERR_CUDA, std::string(what) + ": no device error word");
+  return take_code(word, s, what);
 }
 
 SDG_API size_t sdg_linear_mx4_scratch_bytes(const void* x, int M, int K, int64_t ldx, int N) {

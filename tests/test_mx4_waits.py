@@ -88,4 +88,40 @@ def test_stalled_product_rejects_bad_arguments(sdg, cuda):
             "who": 0, "it": 0, "us": 1000, "err": P(err), "st": None}
     call = lambda **k: sdg.lib().sdg_selftest_stalled_linear_mx4(*(base | k).values())
     assert call(form=4) == call(form=0, M=4) == call(who=1) == call(who=2) == call(it=-1) == call(us=0) == call(us=2000001) \
-        == call(err=None) == call(x=None) == call(xs=None) == 2
+        == call(x=None) == call(xs=None) == 2
+
+
+def test_status_reports_products_without_a_word(sdg, cuda):
+    """A product that had no error word of its own: the failure is reported once, by the next status call."""
+    f, M, N, K, _ = STALLED["narrow"]
+    wc, ws = weight(sdg, N, K, 1)
+    xc, xs = sdg.quantize_mx4(rnd(M, K, seed=2, dtype=torch.float16))
+    want = sdg.linear_mx4(xc, wc, ws, xscale=xs)
+    y = torch.empty_like(want)
+    P = sdg._ptr
+    sdg.mx4_status()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    assert sdg.lib().sdg_selftest_stalled_linear_mx4(P(xc), P(xs), M, K, P(wc), P(ws), N, None, P(y), f, 0, 1, 1000, None,
+                                                     side.cuda_stream) == 0
+    behind = sdg.linear_mx4(xc, wc, ws, xscale=xs, stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(behind, want)
+    with pytest.raises(sdg.SdgError) as ei:
+        sdg.mx4_status(stream=side.cuda_stream)
+    assert ei.value.code == SDG_ERR_DEVICE and "0x10" in str(ei.value)
+    sdg.mx4_status()
+    sdg.mx4_status(device=0)
+
+
+def test_status_refuses_a_captured_stream(sdg, cuda):
+    x = torch.zeros(4, device=cuda)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x += 1
+        with pytest.raises(sdg.SdgError) as ei:
+            sdg.mx4_status()
+    assert ei.value.code == 2
+    g.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1).all())
