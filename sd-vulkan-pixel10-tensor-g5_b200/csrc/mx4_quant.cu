@@ -227,6 +227,8 @@ constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 8;         // pixels a thread holds at once
 constexpr int kGnShift = 4;         // pixels that give the shift
 constexpr int kGnPixels = 16;       // least pixels per thread and chunk of an image of several chunks
+constexpr int kGnRun = 2 * kGnPixels;  // pixels that a thread sums about one shift
+static_assert(kGnRun % kGnBatch == 0, "a run is whole batches");
 constexpr int kGnMaxC = 4096;
 constexpr int kGnMaxChunks = 256;
 
@@ -258,9 +260,10 @@ GnPlan gn_plan(int HW, int C) {
   return p;
 }
 
-// A thread sums d and d^2 of its n pixels of a channel, d = x - k with k the mean of its first m = min(n, 4) pixels.
-// (k - mean)^2 <= M2 / m (Cauchy), so sum d^2 <= M2 (1 + n / m) and M2 = sum d^2 - (sum d)^2 / n loses at most the
-// factor 1 + n / m (9 at 32 pixels) to cancellation, whatever the data.
+// A thread takes its pixels of a channel in runs of n <= 32. It sums d and d^2 over a run, d = x - k with k the mean of the
+// run's first m = min(n, 4) pixels. (k - mean)^2 <= M2 / m (Cauchy), so sum d^2 <= M2 (1 + n / m) and M2 = sum d^2 -
+// (sum d)^2 / n loses at most the factor 1 + n / m <= 9 to cancellation, whatever the data. Runs merge by the update of
+// (n, mean, M2) as threads and chunks do; only images of more than kGnMaxChunks units have chunks of several runs.
 template <typename T>
 __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x, int HW, int C, int groups,
                                                                   int chunk, float2* part) {
@@ -278,48 +281,59 @@ __global__ void __launch_bounds__(kGnThreads, 3) mx4_gn_stats_kernel(const T* x,
     const int cnt = p1 - p0 > first ? (p1 - p0 - first + par - 1) / par : 0;  // this thread's pixels
     const T* at = src + (size_t)first * C;
     const size_t step = (size_t)par * C;
-    float2 k[4], s1[4], s2[4];
+    float4* dst = reinterpret_cast<float4*>(acc + (par > 1 ? r * C : 0) + v * 8);
+#pragma unroll 1
+    for (int run = 0; run < cnt; run += kGnRun) {
+      const int n = min(kGnRun, cnt - run);
+      float2 k[4], s1[4], s2[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = s1[e] = s2[e] = make_float2(0.f, 0.f);
-    for (int i0 = 0; i0 < cnt; i0 += kGnBatch) {
-      const int nb = min(kGnBatch, cnt - i0);
-      uint4 raw[kGnBatch];
+      for (int e = 0; e < 4; ++e) k[e] = s1[e] = s2[e] = make_float2(0.f, 0.f);
+      for (int i0 = 0; i0 < n; i0 += kGnBatch) {
+        const int nb = min(kGnBatch, n - i0);
+        uint4 raw[kGnBatch];
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i) {
-        raw[i] = i < nb ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
-        at += step;
-      }
-      if (i0 == 0) {
-#pragma unroll
-        for (int i = 0; i < kGnShift; ++i) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) k[e] = add_f32x2(k[e], MxElem<T>::get2(w[e]));
+        for (int i = 0; i < kGnBatch; ++i) {
+          raw[i] = i < nb ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
+          at += step;
         }
-        const float inv = 1.f / (float)min(kGnShift, nb);
+        if (i0 == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = mul_f32x2(k[e], make_float2(inv, inv));
-      }
+          for (int i = 0; i < kGnShift; ++i) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i) {
-        if (i < nb) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+            for (int e = 0; e < 4; ++e) k[e] = add_f32x2(k[e], MxElem<T>::get2(w[e]));
+          }
+          const float inv = 1.f / (float)min(kGnShift, nb);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 d = sub_f32x2(MxElem<T>::get2(w[e]), k[e]);
-            s1[e] = add_f32x2(s1[e], d);
-            s2[e] = fma_f32x2(d, d, s2[e]);
+          for (int e = 0; e < 4; ++e) k[e] = mul_f32x2(k[e], make_float2(inv, inv));
+        }
+#pragma unroll
+        for (int i = 0; i < kGnBatch; ++i) {
+          if (i < nb) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 d = sub_f32x2(MxElem<T>::get2(w[e]), k[e]);
+              s1[e] = add_f32x2(s1[e], d);
+              s2[e] = fma_f32x2(d, d, s2[e]);
+            }
           }
         }
       }
-    }
-    const float inv = cnt ? 1.f / (float)cnt : 0.f;
-    float4* dst = reinterpret_cast<float4*>(acc + (par > 1 ? r * C : 0) + v * 8);
+      const float inv = 1.f / (float)n;
+      const float f = (float)n / (float)(run + n), g = f * (float)run;  // shares of this run in a merge
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float mx = s1[e].x * inv, my = s1[e].y * inv;
-      dst[e] = make_float4(k[e].x + mx, max_nan(fmaf(-mx, s1[e].x, s2[e].x), 0.f), k[e].y + my,
-                           max_nan(fmaf(-my, s1[e].y, s2[e].y), 0.f));
+      for (int e = 0; e < 4; ++e) {
+        const float mx = s1[e].x * inv, my = s1[e].y * inv;
+        float4 st = make_float4(k[e].x + mx, max_nan(fmaf(-mx, s1[e].x, s2[e].x), 0.f), k[e].y + my,
+                                max_nan(fmaf(-my, s1[e].y, s2[e].y), 0.f));
+        if (run) {  // with the runs before, which this thread left here
+          const float4 o = dst[e];
+          const float dx = st.x - o.x, dy = st.z - o.z;
+          st = make_float4(fmaf(dx, f, o.x), o.y + fmaf(dx * g, dx, st.y), fmaf(dy, f, o.z), o.w + fmaf(dy * g, dy, st.w));
+        }
+        dst[e] = st;
+      }
     }
   }
   __syncthreads();

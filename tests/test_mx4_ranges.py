@@ -1,9 +1,9 @@
-"""MXFP4 operators at the ends of their ranges, against 64 bits: block scales near the ends of the exponent range. The
-tolerances are those that ``test_mx4`` derives."""
+"""MXFP4 operators at the ends of their ranges, against 64 bits: block scales near the ends of the exponent range, very many
+pixels. The tolerances are those that ``test_mx4`` derives, unless a test says otherwise."""
 import pytest
 import torch
 
-from test_mx4 import close, linear_ref, op64, rnd
+from test_mx4 import check_groupnorm, close, linear_ref, op64, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,30 @@ def test_linear_zero_products_of_large_scales(sdg, cuda, M):
     x[:, 40], w[:, 40] = 1.5, 2.0
     y = sdg.linear_mx4(x, *sdg.quantize_mx4(w))
     assert bool((y == 3.0).all())
+
+
+# ------------------------------------------------------------------ GroupNorm of very many pixels
+def test_groupnorm_statistics_of_many_pixels(sdg, cuda):
+    """2^26 pixels: a thread has 1024 of them, and its first four are unlike the rest, which are all alike. Sums of squares
+    about those four's mean would lose 2^8 to cancellation, and roundings of equal terms all go one way: 0.4 % of the variance.
+
+    Bound: a run of 32 pixels is summed with at most 40 roundings, times 9 for the cancellation; 32 runs, 256 rows x 8
+    channels over 8 lanes and 256 chunks over 8 lanes merge with at most 4 roundings a run and one a term, 64 for the rest."""
+    HW, C, part = 1 << 26, 8, 1 << 18
+    x = torch.full((1, HW, C), 2.125, dtype=torch.float16, device=cuda)
+    x.view(HW // part, part, C)[:, :1024] = 250.0
+    tail = 4096
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x[0, -tail:] = (torch.rand(tail, C, generator=g, device=cuda) * 500 - 250).half()
+    pieces = x.view(64, -1)
+    mu = sum(p.double().sum() for p in pieces) / (HW * C)
+    var = sum((p.double() - mu).square().sum() for p in pieces) / (HW * C)
+    mag = sum(p.double().abs().sum() for p in pieces) / (HW * C)
+    got = sdg.groupnorm_mx4(x, torch.ones(C, device=cuda), torch.zeros(C, device=cuda), 1e-5, False, groups=1)
+    rs = torch.rsqrt(var + 1e-5)
+    t = x[0, -tail:].double()
+    y = (t - mu) * rs
+    e_mu = (40 + 4 * 32 + 256 + 32 + 64) * 2.0 ** -24 * mag
+    rel = (9 * 40 + 4 * 32 + 256 + 32 + 64) * 2.0 ** -24 + 2.0 ** -20 + (e_mu * rs) ** 2
+    delta = rs * e_mu + y.abs() * rel + rs * 2.0 ** -23 * (t.abs() + mu.abs()) + 2.0 ** -22 * y.abs()
+    check_groupnorm((got[0][-tail:], got[1][-tail // 128:]), y.cpu().numpy(), delta.cpu().numpy())
