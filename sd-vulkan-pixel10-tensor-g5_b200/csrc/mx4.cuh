@@ -96,7 +96,6 @@ __device__ __forceinline__ void mx_codes(float (&v)[N], uint32_t e, uint32_t (&q
 // ------------------------------------------------------------------ 16/32-bit element types
 template <typename T> struct MxElem;
 template <> struct MxElem<__half> {
-  static constexpr int kVec = 1;  // 16-byte words per eight values
   // fp32 bits of a |value| from its 16 bits (ordered alike, infinities and NaNs on top)
   static __device__ __forceinline__ uint32_t abs_bits(uint32_t h) {
     return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
@@ -110,7 +109,6 @@ template <> struct MxElem<__half> {
   static __device__ __forceinline__ float2 get2(uint32_t w) { return __half22float2(reinterpret_cast<__half2&>(w)); }
 };
 template <> struct MxElem<__nv_bfloat16> {
-  static constexpr int kVec = 1;
   static __device__ __forceinline__ uint32_t abs_bits(uint32_t h) { return h << 16; }
   static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
@@ -123,8 +121,6 @@ template <> struct MxElem<__nv_bfloat16> {
   }
 };
 template <> struct MxElem<float> {
-  static constexpr int kVec = 2;
-  static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ float put(float v) { return v; }
 };
 

@@ -227,10 +227,10 @@ constexpr uint32_t kGRawBytes = kGBM * 128 * 2;  // 128 columns of 16 bits, as t
 
 template <int BN, bool GEGLU, bool FUSE, bool PAIR>
 struct GCfg {
-  static constexpr int kBTiles = (BN + kMxTileRows - 1) / kMxTileRows;  // scale tiles of w per 128 columns of K
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of w in this CTA
   static constexpr uint32_t kABytes = kGBM * 128, kBBytes = kBRows * 128;
-  static constexpr uint32_t kSfBytes = 2 * kMxTileBytes * (1 + kBTiles);
+  static_assert(BN <= kMxTileRows, "one scale tile of w per 128 columns of K");
+  static constexpr uint32_t kSfBytes = 4 * kMxTileBytes;  // two scale tiles of x, two of w
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr int kPW = GEGLU ? 32 : 64;                 // output columns of a panel (64 accumulator columns)
   static constexpr uint32_t kPanelBytes = 32 * kPW * 2;
@@ -243,7 +243,7 @@ struct GCfg {
   static constexpr uint32_t kTail = kEpiWarps * 64 * 4 + 512;  // bias, barriers, TMEM slot
   static constexpr int kStages = (232448 - 1024 - kTail - kEpiWarps * kPanelBytes - kRawRing) / kStageBytes;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kEpiWarps * kPanelBytes + kRawRing + kTail;
-  static constexpr uint32_t kSfCols = 8 + 8 * kBTiles;        // TMEM columns of one stage's scales
+  static constexpr uint32_t kSfCols = 16;                     // TMEM columns of one stage's scales
   static constexpr uint32_t kTmemCols = 2 * BN + 2 * kSfCols <= 256 ? 256 : 512;
   static_assert(2 * BN + 2 * kSfCols <= 512 && kStages >= 3, "tile does not fit");
   static_assert(!FUSE || kGBM == 2 * 4 * kGQuantWarps, "two passes of four rows a warp");
@@ -425,8 +425,6 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
       tn.next();
       const bool ahead = !FUSE && nst > 4 && tn.valid() && tn.n == 0;
       const int m1 = tn.m * TM + rank * kGBM;
-      int wt = 0;  // scale tiles of w that exist below row N (a tile behind N multiplies columns never stored)
-      for (int j = 0; j < C::kBTiles; ++j) wt += n0 + j * kMxTileRows < p.N;
       for (int k = 0; k < nst; ++k, ++it) {
         const int s = it % S;
         ok = __all_sync(0xffffffffu, waits.wait(empty_bar(s), ((it / S) & 1u) ^ 1u, kDevTimeoutEmpty)) && (int)it != stall_it;
@@ -446,16 +444,13 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
             tma_load_2d_pair(dB, &map_w, fb, k * 128, n0 + rank * C::kBRows);
             tma_load_2d_pair(dS + 2 * kMxTileBytes, &map_ws, fb, k * 256, n0 / kMxTileRows);
           } else {
-            mbar_arrive_expect_tx(full_bar(s), FUSE ? C::kBBytes + sfb * wt : C::kABytes + C::kBBytes + sfb * (1 + wt));
+            mbar_arrive_expect_tx(full_bar(s), FUSE ? C::kBBytes + sfb : C::kABytes + C::kBBytes + 2 * sfb);
             if constexpr (!FUSE) {
               tma_load_2d(dA, &map_x, full_bar(s), k * 128, m0);
               bulk_load(dS, xs + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
             }
             tma_load_2d(dB, &map_w, full_bar(s), k * 128, n0);
-#pragma unroll
-            for (int j = 0; j < C::kBTiles; ++j)
-              if (j < wt)
-                bulk_load(dS + (1 + j) * 2 * kMxTileBytes, ws + ((size_t)j * kts + k * 2) * kMxTileBytes, sfb, full_bar(s));
+            bulk_load(dS + 2 * kMxTileBytes, ws + (size_t)k * 2 * kMxTileBytes, sfb, full_bar(s));
           }
         }
         __syncwarp();
@@ -500,19 +495,17 @@ __global__ void __launch_bounds__(GCfg<BN, ACT == 2, FUSE, PAIR>::kThreads, 1)
           const int nmma = (cols + 63) / 64;
           if (elect_one()) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: 4 columns per tile, per 128 of K]
+            for (int t = 0; t < 2; ++t) {  // TMEM: [x: 4 columns per 128 of K] [w: likewise]
               if (t < nkt) {
                 copy_scales(sf + 4 * t, ds + (t * kMxTileBytes >> 4));
-#pragma unroll
-                for (int j = 0; j < C::kBTiles; ++j)
-                  copy_scales(sf + 8 + 4 * (t * C::kBTiles + j), ds + ((2 * (1 + j) + t) * kMxTileBytes >> 4));
+                copy_scales(sf + 8 + 4 * t, ds + ((2 + t) * kMxTileBytes >> 4));
               }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (j < nmma)
                 mma(d_tmem, da + 2ull * j, db + 2ull * j, idesc_mxf4(TM, BN, (j & 1) * 2), sf + 4 * (j >> 1),
-                    sf + 8 + 4 * (j >> 1) * C::kBTiles + n_off, (k | j) != 0);
+                    sf + 8 + 4 * (j >> 1) + n_off, (k | j) != 0);
             commit(empty_bar(s));
           }
           __syncwarp();
