@@ -65,3 +65,34 @@ def test_groupnorm_statistics_of_many_pixels(sdg, cuda):
     rel = (9 * 40 + 4 * 32 + 256 + 32 + 64) * 2.0 ** -24 + 2.0 ** -20 + (e_mu * rs) ** 2
     delta = rs * e_mu + y.abs() * rel + rs * 2.0 ** -23 * (t.abs() + mu.abs()) + 2.0 ** -22 * y.abs()
     check_groupnorm((got[0][-tail:], got[1][-tail // 128:]), y.cpu().numpy(), delta.cpu().numpy())
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_element_offsets_past_32_bits(sdg, cuda):
+    """4.4e9 elements: the rows behind element 2^32 of every operator's input and output."""
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("needs 48 GB of device memory")
+    R, K = (1 << 22) + 77, 1056
+    x = torch.randn(R, K, dtype=torch.float16, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1))
+    t0 = R // 128 * 128 - 256          # (whole row tiles)
+    assert t0 * K > 1 << 32
+    tail = x[t0:].clone()
+    want = sdg.quantize_mx4(tail)
+    q = sdg.quantize_mx4(x)
+    assert torch.equal(q[0][t0:], want[0]) and torch.equal(q[1][t0 // 128:], want[1])
+    v = sdg.dequantize_mx4(*q)
+    assert torch.equal(v[t0:], sdg.dequantize_mx4(*want))
+    del v
+    wc, ws = sdg.quantize_mx4(rnd(K, K, seed=2) / K ** 0.5)
+    ref, d = linear_ref(op64(*want, K), op64(wc, ws, K), None, tail, 0)
+    y = sdg.linear_mx4(x, wc, ws, residual=x)
+    close(y[t0:], ref, d)
+    torch.cuda.synchronize()
+    y.zero_()
+    close(sdg.linear_mx4(q[0], wc, ws, residual=x, xscale=q[1], out=y)[t0:], ref, d)
+    del y, q
+    g = x[:1 << 22].view(4, 1 << 20, K)
+    gamma, beta = 1 + 0.2 * rnd(K, seed=3), 0.2 * rnd(K, seed=4)
+    a = sdg.groupnorm_mx4(g, gamma, beta, 1e-5, True)
+    b = sdg.groupnorm_mx4(g[3:].clone(), gamma, beta, 1e-5, True)
+    assert torch.equal(a[0][3 << 20:], b[0]) and torch.equal(a[1][(3 << 20) // 128:], b[1])
