@@ -330,7 +330,8 @@ SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M,
 /* The same with x [M, K] of type dtype (row stride ldx elements), quantised on the way: in the
  * same launch for few rows and for small products of 16-byte aligned rows (sdg_linear_mx4_scratch_bytes of the same
  * arguments returns 0 and scratch may be NULL), else into scratch of that many bytes, 16-byte aligned, whose contents
- * on entry do not matter. */
+ * on entry do not matter. Beyond few rows, quantising in the same launch saves the host a launch but not the device time:
+ * in a captured graph sdg_quantize_mx4 and sdg_linear_mx4 are faster. */
 SDG_API int sdg_linear_mx4_x(const void* x, int M, int K, int64_t ldx, const uint8_t* wcodes, const uint8_t* wscales,
                              const float* bias, int N, const void* residual, int act, int dtype, void* y, void* scratch,
                              size_t scratch_bytes, int* err_word, void* stream);
@@ -354,7 +355,7 @@ SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscale
 
 /* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
  * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to
- * 16 bits in between. C a multiple of 8 and of groups, at most 4096. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
+ * 16 bits in between. C a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW at most 2^30. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
  * of device memory, any contents. Deterministic; an image's result does not depend on the batch. */
 SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, int groups, const float* gamma,
                               const float* beta, float eps, int silu, uint8_t* codes, uint8_t* scales,

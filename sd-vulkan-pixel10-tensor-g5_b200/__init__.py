@@ -463,7 +463,8 @@ def upsample_conv3x3(x, wp, bias4, out=None, workspace=None, err_word=None, stre
 # A matrix [rows, K] is (codes, scales): codes uint8 [rows, Kp/2] (Kp = K rounded up to 32), scales uint8
 # [ceil(rows/128), ceil(Kp/128), 512]; the layout is described in include/sdg.h. Every tensor of a call lives on
 # one CUDA device, which need not be the current one; the call runs on that device's current stream, or on
-# ``stream`` (a raw handle of a stream of that device).
+# ``stream`` (a raw handle of a stream of that device). As with every tensor that another stream uses, the caller keeps the
+# arguments alive until the work on ``stream`` is done.
 _torch = None
 _mx4_types: Dict[object, int] = {}
 
@@ -655,7 +656,8 @@ def mx4_status(device=None, stream=None) -> None:
 
 def groupnorm_mx4(x, gamma, beta, eps: float, silu: bool, groups: int = 32, out=None, stats=None, stream=None):
     """GroupNorm (+ SiLU) of channels-last x [B, HW, C] fp16 / bf16, quantised as it is written: the MXFP4 operand
-    (codes, scales) of the matrix [B * HW, C]. ``out``: the pair to write into."""
+    (codes, scales) of the matrix [B * HW, C]. C is a multiple of 8 and of ``groups``, at most 4096, and B at most 65535.
+    ``out``: the pair to write into; ``stats``: fp32 scratch of sdg_groupnorm_mx4_scratch_bytes."""
     if stream is not None:
         return _mx4_on(stream, x, lambda: groupnorm_mx4(x, gamma, beta, eps, silu, groups, out, stats))
     T = _mx4_torch()

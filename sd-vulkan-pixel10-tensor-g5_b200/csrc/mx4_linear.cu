@@ -826,8 +826,9 @@ cudaError_t gemm_bn(const Mx4LinearArgs& a, int* err, cudaStream_t s) {
 
 // The fused form while a block quantises at most this many stages (256 columns of 128 rows, about 1.3 us each). Measured
 // on B200, fused against quantise + product: one eager call 12.3 against 16.4 us (the second launch and the scratch's
-// allocation cost the host 4 us), the device alone 154 x 2560 x 768 7.9 / 5.2 us, 8192 x 320 x 320 10.9 / 7.2 us; beyond
-// six stages the device time passes the host's.
+// allocation cost the host 4 us), the device alone 154 x 2560 x 768 7.9 / 5.2 us, 8192 x 320 x 320 11.0 / 7.2 us; beyond
+// six stages the device time passes the host's. A caller whose host time does not count (a captured graph) quantises x
+// first and passes the operand.
 constexpr long long kFuseStages = 6;
 
 // Few rows run on the CUDA cores, as long as their operand fits 48 KB of shared memory.
