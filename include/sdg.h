@@ -320,9 +320,9 @@ SDG_API int sdg_dequantize_mx4(const uint8_t* codes, const uint8_t* scales, int 
 
 /* y[M,N] = act(x w^T + bias + residual) for MXFP4 x [M, K] and w [N, K], fp32 accumulation. bias [N] fp32
  * (may be NULL); residual [M, N] and y of type dtype (SDG_F16 or SDG_BF16), 16-byte aligned; y may be the
- * residual itself, and overlaps no other argument. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of 16 as for sdg_linear,
- * y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above; without one, sdg_mx4_status tells
- * whether the product completed. */
+ * residual itself, and overlaps no other argument. act: 0 none, 1 SiLU, 2 GEGLU (w rows and bias interleaved in groups of
+ * 16 as for sdg_linear, y is [M, N/2], no residual). N a multiple of 8 (GEGLU: 32). err_word as for the operators above;
+ * without one, sdg_mx4_status tells whether the product completed. */
 SDG_API int sdg_linear_mx4(const uint8_t* xcodes, const uint8_t* xscales, int M, int K, const uint8_t* wcodes,
                            const uint8_t* wscales, const float* bias, int N, const void* residual, int act, int dtype,
                            void* y, int* err_word, void* stream);
@@ -355,8 +355,8 @@ SDG_API int sdg_selftest_stalled_linear_mx4(const void* x, const uint8_t* xscale
 
 /* GroupNorm(groups) (+ SiLU) of channels-last x [B, HW, C] (SDG_F16 or SDG_BF16, 16-byte aligned) written as
  * the MXFP4 operand [B*HW, C] of the product that follows: the fp32 result is quantised without a rounding to
- * 16 bits in between. C a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW at most 2^30. stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes
- * of device memory, any contents. Deterministic; an image's result does not depend on the batch. */
+ * 16 bits in between. C a multiple of 8 and of groups, at most 4096; B at most 65535, B * HW at most 2^30.
+ * stats_scratch: sdg_groupnorm_mx4_scratch_bytes() bytes of device memory, any contents. Deterministic; an image's result does not depend on the batch. */
 SDG_API int sdg_groupnorm_mx4(const void* x, int dtype, int B, int HW, int C, int groups, const float* gamma,
                               const float* beta, float eps, int silu, uint8_t* codes, uint8_t* scales,
                               float* stats_scratch, void* stream);

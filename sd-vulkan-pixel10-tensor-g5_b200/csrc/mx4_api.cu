@@ -17,8 +17,8 @@ namespace {
 using sdg::op_fail;
 
 // The word the kernels' bounded waits report to when the caller passes none: zero-initialised device memory of the
-// library, looked up once per device; sdg_mx4_status reads and clears it. The look-up may load the module, so it runs with this thread's
-// stream-capture mode relaxed: a first call inside a capture is fine.
+// library, looked up once per device; sdg_mx4_status reads and clears it. The look-up may load the module, so it runs with
+// this thread's stream-capture mode relaxed: a first call inside a capture is fine.
 static __device__ int g_mx4_err[64];
 std::mutex g_mu;
 int* g_err_dev[64] = {nullptr};

@@ -393,7 +393,7 @@ __device__ __forceinline__ float2 gn_merge(const float2* part, int g, int groups
 }
 
 // y * sigmoid(y) of two values with one reciprocal, 1 / (a b): three MUFU instructions for two values instead of four
-// (the apply kernel would be bound by that pipe). A few fp32 ulps off: the rounding to four bits comes after it, so the
+// (the apply kernel would be bound by that pipe). Off by a few fp32 ulps, and |y| more for y < 0 (the exponent's rounding): the rounding to four bits comes after it, so the
 // approximation must not move values across the E2M1 midpoints more often than fp32 arithmetic does. a and b are
 // capped at 2^63 so that their product stays finite: below y = -43.7 the result is off by up to |y| 2^-63, which is
 // nothing next to a block maximum that is not itself below 2^-40.
