@@ -1,9 +1,10 @@
 """MXFP4 operators at the ends of their ranges, against 64 bits: block scales near the ends of the exponent range, very many
 pixels. The tolerances are those that ``test_mx4`` derives, unless a test says otherwise."""
+import numpy as np
 import pytest
 import torch
 
-from test_mx4 import check_groupnorm, close, linear_ref, op64, rnd
+from test_mx4 import check_groupnorm, close, groupnorm_ref, linear_ref, op64, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +97,22 @@ def test_element_offsets_past_32_bits(sdg, cuda):
     a = sdg.groupnorm_mx4(g, gamma, beta, 1e-5, True)
     b = sdg.groupnorm_mx4(g[3:].clone(), gamma, beta, 1e-5, True)
     assert torch.equal(a[0][3 << 20:], b[0]) and torch.equal(a[1][(3 << 20) // 128:], b[1])
+
+
+# ------------------------------------------------------------------ SiLU far below zero
+@pytest.mark.parametrize("HW", [8, 512])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_groupnorm_silu_of_very_negative_blocks(sdg, cuda, HW, dtype):
+    """Blocks whose values are all SiLU of -20 to -84: tiny, but an operand's exponent follows them.
+
+    There SiLU is y exp(y) but for 2^-28, its relative slope 1 + 1 / y: an error d of y counts 1.1 d, the exponent's rounding
+    |y| 2^-24 and the function 2^-21, each relative."""
+    C = 320
+    x = rnd(2, HW, C, seed=6, dtype=dtype)
+    gamma = 1 + 0.2 * rnd(C, seed=1)
+    beta = -24.0 - 56.0 * (torch.arange(C, device=cuda) // 32) / 9
+    y, d = groupnorm_ref(x, gamma, beta, 1e-5, False, 32)
+    assert y.max() < -16 and y.min() > -87
+    ref = y / (1 + np.exp(-y))
+    delta = np.abs(ref) * (1.1 * d + np.abs(y) * 2.0 ** -23 + 2.0 ** -21)
+    check_groupnorm(sdg.groupnorm_mx4(x, gamma, beta, 1e-5, True), ref, delta)
